@@ -288,7 +288,7 @@ class CacheManager:
             if key not in keys:
                 keys[key] = len(out)
                 out.append(0)
-            out[keys[key]] += pages.bytes_per_token(dtype) * page_size
+            out[keys[key]] += pages.bytes_per_page(page_size, dtype)
         return out
 
     # -- bookkeeping -----------------------------------------------------------------------

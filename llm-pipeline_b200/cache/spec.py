@@ -10,6 +10,7 @@ the same ``group_key()`` share page ids and block tables. The manager, the memor
 benchmark read sizes from the spec alone (``elements_per_token``, ``bytes_per_token``).
 
 * ``KVPagesSpec``: keys and values of attention, page ``[2, kv_heads, page_size, head_dim]``.
+* ``KV8PagesSpec``: keys and values of attention in 8 bits with a scale for each page and head, page ``[bytes]``.
 * ``HeadRowPagesSpec``: one row of ``row_size`` entries per key/value head and token (keys and values of different
   widths, or several keys, packed side by side), page ``[kv_heads, page_size, row_size]``.
 * ``TokenPagesSpec``: any payload of a fixed shape per token, page ``[page_size, *token_shape]``
@@ -65,6 +66,9 @@ class PagesSpec:
     def bytes_per_token(self, cache_dtype: torch.dtype) -> int:
         return self.elements_per_token() * torch.empty((), dtype=self.dtype or cache_dtype).element_size()
 
+    def bytes_per_page(self, page_size: int, cache_dtype: torch.dtype) -> int:
+        return self.bytes_per_token(cache_dtype) * page_size
+
 
 @dataclass(frozen=True)
 class KVPagesSpec(PagesSpec):
@@ -77,6 +81,35 @@ class KVPagesSpec(PagesSpec):
 
     def group_key(self):
         return ("kv", self.num_kv_heads, self.head_dim, self.window)
+
+
+def kv8_page_bytes(num_kv_heads: int, page_size: int, head_dim: int) -> int:
+    """Bytes of a page of keys and values in 8 bits: the values, a scale byte per head for keys and for values, padding to a
+    multiple of 128."""
+    return -(-(2 * num_kv_heads * (page_size * head_dim + 1)) // 128) * 128
+
+
+@dataclass(frozen=True)
+class KV8PagesSpec(PagesSpec):
+    """Keys and values in e4m3: a page is ``[2][kv_heads][page_size][head_dim]`` bytes, then ``[2][kv_heads]`` scale bytes (byte
+    e: 2^(e - 127), 0: 0), padded."""
+
+    num_kv_heads: int
+    head_dim: int
+    window: Optional[int] = None
+    dtype = torch.uint8
+
+    def page_shape(self, page_size: int) -> Tuple[int, ...]:
+        return (kv8_page_bytes(self.num_kv_heads, page_size, self.head_dim),)
+
+    def group_key(self):
+        return ("kv8", self.num_kv_heads, self.head_dim, self.window)
+
+    def elements_per_token(self) -> int:
+        return 2 * self.num_kv_heads * self.head_dim           # the scales and the padding belong to the page
+
+    def bytes_per_page(self, page_size: int, cache_dtype: torch.dtype) -> int:
+        return self.page_shape(page_size)[0]
 
 
 @dataclass(frozen=True)

@@ -336,7 +336,7 @@ __global__ void qkv_post_kernel(T* __restrict__ qkv, const void* __restrict__ bi
                                 const void* __restrict__ q_w, const void* __restrict__ k_w, int w_bf16,
                                 float eps, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
                                 int rotary_dim, const int* __restrict__ slots, T* __restrict__ pages,
-                                int nq, int nkv, int d, int page_size) {
+                                int nq, int nkv, int d, int page_size, int keep_rows) {
     extern __shared__ float head_smem[];           // [QKV_WARPS][d]
     pdl_trigger();                                 // the attention kernel may start fetching keys of earlier steps
     pdl_wait();                                    // the projection is complete
@@ -381,7 +381,7 @@ __global__ void qkv_post_kernel(T* __restrict__ qkv, const void* __restrict__ bi
             __syncwarp();
         }
         T* dst = nullptr;
-        if (is_q) {
+        if (is_q || keep_rows) {
             dst = src;
         } else if (pages && slot >= 0) {
             const int kvh = is_k ? h - nq : h - nq - nkv;
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(QKV_WARPS * 32)
 qkv_post_d128_kernel(T* __restrict__ qkv, const void* __restrict__ bias, int bias_bf16,
                      const void* __restrict__ q_w, const void* __restrict__ k_w, int w_bf16, float eps,
                      const float* __restrict__ cos_t, const float* __restrict__ sin_t, const int* __restrict__ slots,
-                     T* __restrict__ pages, int nq, int nkv, int page_size) {
+                     T* __restrict__ pages, int nq, int nkv, int page_size, int keep_rows) {
     constexpr int D = 128;
     pdl_trigger();                                 // the attention kernel may start fetching keys of earlier steps
     const int n = blockIdx.x;
@@ -507,7 +507,7 @@ qkv_post_d128_kernel(T* __restrict__ qkv, const void* __restrict__ bias, int bia
                 for (int e = 0; e < 8; ++e) v[u][e] = v[u][e] * c[e] + other[e] * s[e];
             }
             T* dst = nullptr;
-            if (is_q) {
+            if (is_q || (keep_rows && live)) {
                 dst = row + (size_t)h * D + e0;
             } else if (live && pages && slot >= 0) {
                 const int kvh = is_k ? h - nq : h - nq - nkv;
@@ -522,7 +522,7 @@ qkv_post_d128_kernel(T* __restrict__ qkv, const void* __restrict__ bias, int bia
 LLMP_API int llmp_qkv_post(void* qkv, int dtype, const void* bias, int bias_dtype, const void* q_w, const void* k_w,
                            int w_dtype, float eps, const float* cos_t, const float* sin_t, int rotary_dim,
                            const int* slots, void* pages, int N, int nq, int nkv, int d, int page_size,
-                           cudaStream_t stream) {
+                           int keep_rows, cudaStream_t stream) {
     if (N <= 0) return 0;
     LLMP_REQUIRE(nq > 0 && nkv >= 0 && d > 0, "qkv_post: bad sizes nq=%d nkv=%d d=%d", nq, nkv, d);
     LLMP_REQUIRE(rotary_dim >= 0 && rotary_dim <= d && rotary_dim % 2 == 0,
@@ -545,11 +545,11 @@ LLMP_API int llmp_qkv_post(void* qkv, int dtype, const void* bias, int bias_dtyp
         if (dtype == LLMP_F32)
             qkv_post_d128_kernel<float><<<grid128, QKV_WARPS * 32, 0, stream>>>(
                 (float*)qkv, bias, bias_dtype == LLMP_BF16, q_w, k_w, w_dtype == LLMP_BF16, eps, cos_t, sin_t, slots,
-                (float*)pages, nq, nkv, page_size);
+                (float*)pages, nq, nkv, page_size, keep_rows);
         else
             llmp_launch_dependent(qkv_post_d128_kernel<bf16>, grid128, dim3(QKV_WARPS * 32), 0, stream,
                                   (bf16*)qkv, bias, bias_dtype == LLMP_BF16, q_w, k_w, w_dtype == LLMP_BF16, eps, cos_t, sin_t,
-                                  slots, (bf16*)pages, nq, nkv, page_size);
+                                  slots, (bf16*)pages, nq, nkv, page_size, keep_rows);
         return llmp_check_launch("qkv_post");
     }
     dim3 grid(N, head_blocks);
@@ -558,7 +558,7 @@ LLMP_API int llmp_qkv_post(void* qkv, int dtype, const void* bias, int bias_dtyp
 #define QKV_LAUNCH(T, V)                                                                                              \
     qkv_post_kernel<T, V><<<grid, QKV_WARPS * 32, smem, stream>>>(                                                    \
         (T*)qkv, bias, bias_dtype == LLMP_BF16, q_w, k_w, w_dtype == LLMP_BF16, eps, cos_t, sin_t, rotary_dim, slots, \
-        (T*)pages, nq, nkv, d, page_size)
+        (T*)pages, nq, nkv, d, page_size, keep_rows)
     if (dtype == LLMP_F32) {
         if (vec == 4) QKV_LAUNCH(float, 4); else if (vec == 2) QKV_LAUNCH(float, 2); else QKV_LAUNCH(float, 1);
     } else {

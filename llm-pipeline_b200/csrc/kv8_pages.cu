@@ -1,0 +1,292 @@
+// Writing and unpacking pages of 8-bit keys and values (kv8.cuh), and copying pages of any cache.
+#include "kv8.cuh"
+
+#define KV8_WARPS 4
+
+// ---- storing -----------------------------------------------------------------------------------------------------------
+// Rows of k and v [tokens, nkv * d] go to their slots (page * page_size + offset; negative: nowhere). A run is the
+// consecutive rows of one page (rows without a slot between them aside). Per run and block (keys or values of one head):
+//   need = smallest scale that holds the run's largest finite magnitude
+//   e    = need, or the block's scale where that is larger and the run begins behind the page's first token
+//   values held before the run's first offset, if e has grown:  q <- nearest(q * 2^(old - e))
+//   the run's values:  q <- nearest(x * 2^(127 - e)), infinities and NaN to "no number"
+// One warp owns a run of a block, so nothing is shared; rows of one page that are not neighbours would be two runs that
+// write the same block at once. What lies behind the run in its page stays as it is.
+struct StoreParams {
+    const void* k;
+    const void* v;
+    const int* slots;
+    unsigned char* pages;
+    long k_stride, v_stride, page_bytes;
+    int N, nkv, d, page_size, num_pages, rows_per_block, wide;
+};
+
+template <typename T> __device__ __forceinline__ void kv8_load4(const T* p, int wide, float (&x)[4]) {
+    if (wide) {
+        if (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(p);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(p);
+            x[0] = __uint_as_float(a.x << 16); x[1] = __uint_as_float(a.x & 0xffff0000u);
+            x[2] = __uint_as_float(a.y << 16); x[3] = __uint_as_float(a.y & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = to_float(p[i]);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(KV8_WARPS * 32) kv8_store_kernel(const StoreParams p) {
+    pdl_trigger();
+    pdl_wait();                                                  // the rows, and what the pages hold, are complete
+    const int lane = threadIdx.x & 31;
+    const int unit = blockIdx.y * KV8_WARPS + (threadIdx.x >> 5);        // keys or values of one head
+    if (unit >= 2 * p.nkv) return;
+    const bool values = unit >= p.nkv;
+    const T* src = reinterpret_cast<const T*>(values ? p.v : p.k) + (size_t)(values ? unit - p.nkv : unit) * p.d;
+    const size_t stride = values ? p.v_stride : p.k_stride;
+    const int slots_end = p.num_pages * p.page_size, quads = p.d / 4;
+    auto slot_of = [&](int row) {                                // no slot beyond the pages is written to
+        const int s = p.slots[row];
+        return s < slots_end ? s : -1;
+    };
+    const int row_end = min(p.N, (int)(blockIdx.x + 1) * p.rows_per_block);
+    for (int first = blockIdx.x * p.rows_per_block; first < row_end; ++first) {
+        const int slot = slot_of(first);
+        if (slot < 0) continue;
+        const int page = slot / p.page_size;
+        int before = first - 1;
+        while (before >= 0 && slot_of(before) < 0) --before;
+        if (before >= 0 && slot_of(before) / p.page_size == page) continue;      // in the middle of a run
+        int end = first + 1, lowest = slot % p.page_size;
+        for (; end < p.N; ++end) {
+            const int s = slot_of(end);
+            if (s < 0) continue;
+            if (s / p.page_size != page) break;
+            lowest = min(lowest, s % p.page_size);
+        }
+        unsigned char* block = p.pages + (size_t)page * p.page_bytes + (size_t)unit * p.page_size * p.d;
+        unsigned char* scale = p.pages + (size_t)page * p.page_bytes + (size_t)2 * p.nkv * p.page_size * p.d + unit;
+        const int count = (end - first) * quads;
+        float amax = 0.f;
+        for (int i = lane; i < count; i += 32) {
+            const int row = first + i / quads;
+            if (slot_of(row) < 0) continue;
+            float x[4];
+            kv8_load4(src + (size_t)row * stride + (i % quads) * 4, p.wide, x);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float a = fabsf(x[c]);
+                if (a < INFINITY) amax = fmaxf(amax, a);         // neither infinities nor NaN
+            }
+        }
+        amax = warp_max(amax);
+        int e = kv8_needed(amax);
+        if (lowest > 0) {
+            const int old = *scale;
+            if (old >= e) {
+                e = old;
+            } else {                                             // the tokens before the run move to the larger scale
+                const float down = kv8_power(max(old - e, -126));
+                for (int i = lane; i < lowest * quads; i += 32) {
+                    unsigned* at = reinterpret_cast<unsigned*>(block) + i;
+                    float q[4];
+                    kv8_unpack4(*at, q);
+                    *at = kv8_pack4(q[0] * down, q[1] * down, q[2] * down, q[3] * down);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) *scale = (unsigned char)e;
+        const float up = kv8_power(127 - e);
+        for (int i = lane; i < count; i += 32) {
+            const int row = first + i / quads, c = (i % quads) * 4;
+            const int s = slot_of(row);
+            if (s < 0) continue;
+            float x[4];
+            kv8_load4(src + (size_t)row * stride + c, p.wide, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = fabsf(x[j]) < INFINITY ? x[j] * up : __int_as_float(0x7fffffff);
+            *reinterpret_cast<unsigned*>(block + (size_t)(s % p.page_size) * p.d + c) = kv8_pack4(x[0], x[1], x[2], x[3]);
+        }
+    }
+}
+
+static int kv8_check_sizes(const char* what, const void* pages, int num_pages, int nkv, int d, int page_size) {
+    LLMP_REQUIRE(nkv > 0 && num_pages > 0 && page_size > 0, "%s: bad sizes (%d heads, %d pages of %d tokens)", what, nkv, num_pages, page_size);
+    LLMP_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, "%s: head size %d is not a multiple of 16 in 16..256", what, d);
+    LLMP_REQUIRE(((size_t)pages % 16) == 0, "%s: pages must be 16-byte aligned", what);
+    LLMP_REQUIRE((long)num_pages * page_size < (1L << 31), "%s: token slots pass 32 bits", what);
+    return 0;
+}
+
+LLMP_API long llmp_kv8_page_bytes(int nkv, int page_size, int d) { return kv8_page_bytes(nkv, page_size, d); }
+
+LLMP_API int llmp_kv8_store(const void* k, long k_stride, const void* v, long v_stride, int dtype, const int* slots, void* pages,
+                            int num_pages, int N, int nkv, int d, int page_size, cudaStream_t stream) {
+    if (N <= 0) return 0;
+    if (kv8_check_sizes("kv8_store", pages, num_pages, nkv, d, page_size)) return 1;
+    StoreParams p;
+    p.k = k; p.v = v; p.slots = slots; p.pages = (unsigned char*)pages; p.k_stride = k_stride; p.v_stride = v_stride;
+    p.page_bytes = kv8_page_bytes(nkv, page_size, d); p.N = N; p.nkv = nkv; p.d = d; p.page_size = page_size; p.num_pages = num_pages;
+    const size_t quad = dtype == LLMP_F32 ? 16 : 8;
+    p.wide = ((size_t)k % quad) == 0 && ((size_t)v % quad) == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
+    p.rows_per_block = N <= 256 ? 1 : 16;
+    const dim3 grid((N + p.rows_per_block - 1) / p.rows_per_block, (2 * nkv + KV8_WARPS - 1) / KV8_WARPS);
+    LLMP_REQUIRE(grid.y <= 65535, "kv8_store: too many heads");
+    if (dtype == LLMP_F32) llmp_launch_dependent(kv8_store_kernel<float>, grid, dim3(KV8_WARPS * 32), 0, stream, p);
+    else llmp_launch_dependent(kv8_store_kernel<bf16>, grid, dim3(KV8_WARPS * 32), 0, stream, p);
+    return llmp_check_launch("kv8_store");
+}
+
+// ---- unpacking ---------------------------------------------------------------------------------------------------------
+// Page i of out [n, 2, nkv, page_size, d] gets the values of the page in entry index[i] of the block tables [R, table_stride];
+// zeros for tokens behind the request's context and for a missing page. 16 values a thread, exact in either type.
+struct GatherParams {
+    const unsigned char* pages;
+    const int* tables;
+    const int* ctx_len;
+    const int* index;
+    void* out;
+    long page_bytes;
+    int n, table_stride, entries, nkv, d, page_size, num_pages;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) kv8_gather_kernel(const GatherParams p) {
+    pdl_trigger();
+    pdl_wait();
+    const int i = blockIdx.x;
+    const int entry = p.index[i];
+    const bool known = entry >= 0 && entry < p.entries;
+    int page = known ? p.tables[entry] : -1;
+    if (page >= p.num_pages) page = -1;
+    const int token0 = known ? entry % p.table_stride * p.page_size : 0;
+    const int there = page >= 0 ? p.ctx_len[entry / p.table_stride] - token0 : 0;      // tokens of the page that exist
+    const unsigned char* src = p.pages + (size_t)(page < 0 ? 0 : page) * p.page_bytes;
+    const int pieces = p.d / 16, body = 2 * p.nkv * p.page_size * pieces;
+    T* out = reinterpret_cast<T*>(p.out) + (size_t)i * body * 16;
+    for (int at = blockIdx.y * blockDim.x + threadIdx.x; at < body; at += gridDim.y * blockDim.x) {
+        const int row = at / pieces;                             // (keys or values, head, token)
+        const bool live = row % p.page_size < there;
+        float f[16];
+        if (live) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(src + (size_t)at * 16);
+            const float s = kv8_scale(src[(size_t)body * 16 + row / p.page_size]);
+            const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float q[4];
+                kv8_unpack4(w[c], q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[c * 4 + j] = q[j] * s;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[j] = 0.f;
+        }
+        T* dst = out + (size_t)at * 16;
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) reinterpret_cast<float4*>(dst)[c] = make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                unsigned w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(f[8 * c + 2 * j], f[8 * c + 2 * j + 1]);
+                    w[j] = *reinterpret_cast<const unsigned*>(&h);
+                }
+                reinterpret_cast<uint4*>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
+LLMP_API int llmp_kv8_gather(const void* pages, int num_pages, const int* tables, int R, int table_stride, const int* ctx_len,
+                             const int* index, int n, void* out, int dtype, int nkv, int d, int page_size, cudaStream_t stream) {
+    if (n <= 0) return 0;
+    if (kv8_check_sizes("kv8_gather", pages, num_pages, nkv, d, page_size)) return 1;
+    LLMP_REQUIRE(((size_t)out % 16) == 0, "kv8_gather: the output must be 16-byte aligned");
+    LLMP_REQUIRE(table_stride > 0 && (long)R * table_stride < (1L << 31), "kv8_gather: bad block tables");
+    LLMP_REQUIRE(2L * nkv * page_size * d < (1L << 31), "kv8_gather: a page of %d tokens is too large", page_size);
+    GatherParams p;
+    p.pages = (const unsigned char*)pages; p.tables = tables; p.ctx_len = ctx_len; p.index = index; p.out = out;
+    p.page_bytes = kv8_page_bytes(nkv, page_size, d); p.n = n; p.table_stride = table_stride; p.entries = R * table_stride;
+    p.nkv = nkv; p.d = d; p.page_size = page_size; p.num_pages = num_pages;
+    const long pieces = 2L * nkv * page_size * d / 16;
+    const long blocks = (pieces + 1023) / 1024;                  // four pieces a thread
+    const dim3 grid(n, (unsigned)(blocks < 64 ? blocks : 64));
+    if (dtype == LLMP_F32) llmp_launch_dependent(kv8_gather_kernel<float>, grid, dim3(256), 0, stream, p);
+    else llmp_launch_dependent(kv8_gather_kernel<bf16>, grid, dim3(256), 0, stream, p);
+    return llmp_check_launch("kv8_gather");
+}
+
+// ---- copying pages -------------------------------------------------------------------------------------------------------
+// Page src[i] to page dst[i] in every one of a few caches; no destination is a source or another destination (the caller
+// checks), so the copies are independent. The list travels in the launch's parameters: nothing to upload, nothing that has to
+// outlive the launch.
+#define COPY_TENSORS 48
+#define COPY_PAIRS 384
+struct CopyParams {
+    unsigned char* base[COPY_TENSORS];
+    int src[COPY_PAIRS], dst[COPY_PAIRS];
+    long page_bytes;
+    int wide;
+};
+#define COPY_BLOCK_BYTES 16384
+
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+    unsigned char* base = p.base[blockIdx.z];
+    const unsigned char* src = base + (size_t)p.src[blockIdx.y] * p.page_bytes;
+    unsigned char* dst = base + (size_t)p.dst[blockIdx.y] * p.page_bytes;
+    const long at = (long)blockIdx.x * COPY_BLOCK_BYTES;
+    const int bytes = (int)(p.page_bytes - at < COPY_BLOCK_BYTES ? p.page_bytes - at : COPY_BLOCK_BYTES);
+    pdl_trigger();
+    pdl_wait();
+    if (p.wide) {
+        uint4 v[COPY_BLOCK_BYTES / 4096];
+#pragma unroll
+        for (int i = 0; i < COPY_BLOCK_BYTES / 4096; ++i) {
+            const int o = (i * 256 + threadIdx.x) * 16;
+            if (o < bytes) v[i] = *reinterpret_cast<const uint4*>(src + at + o);
+        }
+#pragma unroll
+        for (int i = 0; i < COPY_BLOCK_BYTES / 4096; ++i) {
+            const int o = (i * 256 + threadIdx.x) * 16;
+            if (o < bytes) *reinterpret_cast<uint4*>(dst + at + o) = v[i];
+        }
+    } else {
+        for (int o = threadIdx.x; o < bytes; o += 256) dst[at + o] = src[at + o];
+    }
+}
+
+LLMP_API int llmp_copy_pages_max_tensors() { return COPY_TENSORS; }
+LLMP_API int llmp_copy_pages_max_pairs() { return COPY_PAIRS; }
+
+// bases: host array of `tensors` device pointers; src, dst: host arrays of `pairs` page numbers.
+LLMP_API int llmp_copy_pages(const void* const* bases, int tensors, long page_bytes, const int* src, const int* dst, int pairs,
+                             cudaStream_t stream) {
+    if (tensors <= 0 || pairs <= 0 || page_bytes <= 0) return 0;
+    LLMP_REQUIRE(tensors <= COPY_TENSORS && pairs <= COPY_PAIRS, "copy_pages: %d caches and %d pages are more than a launch takes", tensors, pairs);
+    CopyParams p;
+    bool wide = page_bytes % 16 == 0;
+    for (int i = 0; i < tensors; ++i) {
+        p.base[i] = (unsigned char*)const_cast<void*>(bases[i]);
+        wide = wide && ((size_t)bases[i] % 16) == 0;
+    }
+    for (int i = 0; i < pairs; ++i) {
+        p.src[i] = src[i];
+        p.dst[i] = dst[i];
+    }
+    p.page_bytes = page_bytes;
+    p.wide = wide;
+    const long chunks = (page_bytes + COPY_BLOCK_BYTES - 1) / COPY_BLOCK_BYTES;
+    LLMP_REQUIRE(chunks < (1L << 31), "copy_pages: a page is too large");
+    const dim3 grid((unsigned)chunks, pairs, tensors);
+    llmp_launch_dependent(copy_pages_kernel, grid, dim3(256), 0, stream, p);
+    return llmp_check_launch("copy_pages");
+}

@@ -53,7 +53,8 @@ class _CacheViews:
     def view(self, cache_id: int, writes: bool) -> LayerCache:
         group = self.cache.group_of_cache.get(cache_id)
         pages = self.cache.pages_tensor(cache_id) if group is not None else None
-        return LayerCache(pages=pages, group=group, state=self.cache.state_tensor(cache_id), writes=writes)
+        return LayerCache(pages=pages, group=group, state=self.cache.state_tensor(cache_id), writes=writes,
+                          page_size=self.cache.page_size)
 
 
 class _DecodeGraph:

@@ -10,7 +10,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
-from ..cache.spec import PagesSpec, StateSpec
+from ..cache.spec import KV8PagesSpec, PagesSpec, StateSpec
 from ..config.base import ModelSpec, PartSpec
 from ..ops.linear import begin_step
 from ..ops.timing import nvtx_range
@@ -85,14 +85,22 @@ class Model:
         limits = [n for n in limits if n is not None]
         return min(limits) if limits else None
 
-    def cache_specs(self) -> List[Tuple[Optional[PagesSpec], Optional[StateSpec]]]:
+    def cache_specs(self, kv_cache_dtype: Optional[str] = None) -> List[Tuple[Optional[PagesSpec], Optional[StateSpec]]]:
         """Per cache id, what the layer that owns it asks of the cache manager; last, what the embedding asks, if it
-        carries something from token to token."""
+        carries something from token to token. ``kv_cache_dtype``: None for the model's type, "e4m3" for keys and values in 8
+        bits in the layers whose mixer has such a form (an error if none has)."""
+        if kv_cache_dtype not in (None, "e4m3"):
+            raise ValueError(f"keys and values are held in the model's type (None) or in 8 bits (\"e4m3\"), not {kv_cache_dtype!r}")
         count = max((e.cache for e in self.schedule), default=-1) + 1
         specs: List[Tuple[Optional[PagesSpec], Optional[StateSpec]]] = [(None, None)] * count
         for cache_id, index in self._owner.items():
             block = self.blocks[self.schedule[index].layer]
-            specs[cache_id] = (block.mixer.cache_spec(), block.state_spec())
+            pages = block.mixer.cache_spec()
+            if kv_cache_dtype is not None:
+                pages = block.mixer.cache_spec_8bit() or pages
+            specs[cache_id] = (pages, block.state_spec())
+        if kv_cache_dtype is not None and not any(isinstance(pages, KV8PagesSpec) for pages, _state in specs):
+            raise ValueError(f"no layer of this {self.spec.architecture} model can hold its keys and values in 8 bits")
         if self.embedding_cache is not None:
             specs.append((None, self.embedding.state_spec()))
         return specs
@@ -172,7 +180,7 @@ class Model:
             cache = caches.view(entry.cache, writes=self._owner[entry.cache] == index)
             if entry.pages_from is not None:
                 other = caches.view(entry.pages_from, writes=False)
-                cache = LayerCache(pages=other.pages, group=other.group, state=cache.state, writes=False)
+                cache = LayerCache(pages=other.pages, group=other.group, state=cache.state, writes=False, page_size=other.page_size)
             with nvtx_range(f"layer {entry.layer} (execution {index})"):
                 self.blocks[entry.layer].forward(stream, ctx, cache)
 

@@ -14,6 +14,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
+from ..cache.spec import kv8_page_bytes
 from .build import library
 
 F32, BF16 = 0, 1
@@ -40,7 +41,7 @@ _SIGNATURES = {
     "llmp_embedding_bigram": [_P, _P, _P, _I, _P, _P, _P, _P, _P, _L, _L, _L, _P, _I, _I, _I, _P],
     "llmp_rope_tables": [_P, _P, _F, _P, _P, _I, _I, _P],
     "llmp_add_rmsnorm": [_P, _P, _P, _I, _P, _I, _F, _P, _I, _P, _I, _I, _P],
-    "llmp_qkv_post": [_P, _I, _P, _I, _P, _P, _I, _F, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P],
+    "llmp_qkv_post": [_P, _I, _P, _I, _P, _P, _I, _F, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "llmp_swiglu": [_P, _P, _I, _I, _I, _P],
     "llmp_gemm_simt": [_P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _L, _L, _L, _P],
     "llmp_gemm_skinny": [_P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _P],
@@ -118,6 +119,10 @@ _SIGNATURES = {
     "llmp_wkv_gate": [_P, _L, _P, _L, _P, _P, _I, _L, _I, _I, _I, _F, _P],
     "llmp_xielu": [_P, _P, _I, _F, _F, _P, _I, _L, _I, _P],
     "llmp_scaled_sum": [_P, _F, _P, _F, _P, _L, _P],
+    "llmp_kv8_store": [_P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _I, _P],
+    "llmp_kv8_gather": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P],
+    "llmp_kv8_decode": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
+    "llmp_copy_pages": [_P, _I, _L, _P, _P, _I, _P],
 }
 _bound = {}
 launch_count = 0   # kernels of this library launched so far (captured launches count once per capture)
@@ -345,13 +350,15 @@ def library_add_product(residual: torch.Tensor, x: torch.Tensor, w: torch.Tensor
 def qkv_post(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, *,
              bias: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
              eps: float, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], rotary_dim: int,
-             slots: Optional[torch.Tensor], pages: Optional[torch.Tensor], page_size: int) -> None:
+             slots: Optional[torch.Tensor], pages: Optional[torch.Tensor], page_size: int, keep_rows: bool = False) -> None:
     """In place on qkv [N, (nq + 2 nkv) d]: bias, per-head RMSNorm of q and k, rotary; k and v are
-    stored to their page slots (pages [P, 2, nkv, page_size, d])."""
+    stored to their page slots (pages [P, 2, nkv, page_size, d]). ``keep_rows``: k and v go back into their rows instead
+    (for a cache of another layout, which a kernel of its own fills from them)."""
     N = qkv.shape[0]
     _need(qkv.is_contiguous() and qkv.shape[1] == (num_heads + 2 * num_kv_heads) * head_dim,
           "qkv must be contiguous [tokens, (heads + 2 kv heads) * head_dim]")
     if pages is not None:
+        _need(not keep_rows, "keys and values go to pages or back into their rows, not both")
         _need(pages.dtype == qkv.dtype and pages.is_contiguous() and
               tuple(pages.shape[1:]) == (2, num_kv_heads, page_size, head_dim), "pages have the wrong layout")
         _need(slots is not None, "a page write needs slots")
@@ -371,7 +378,7 @@ def qkv_post(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int
     _call("llmp_qkv_post", _ptr(qkv), dtype_code(qkv.dtype), _ptr(bias),
           dtype_code(bias.dtype) if bias is not None else F32, _ptr(q_weight), _ptr(k_weight), w_dtype, float(eps),
           _ptr(cos), _ptr(sin), int(rotary_dim), _ptr(slots), _ptr(pages), N, num_heads, num_kv_heads, head_dim,
-          int(page_size), _stream())
+          int(page_size), int(bool(keep_rows)), _stream())
 
 
 def swiglu(gate_up: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
@@ -2291,3 +2298,114 @@ def wkv_gate(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, out: tor
     _call("llmp_wkv_gate", _ptr(o), o.stride(0), _ptr(gate), gate.stride(0), _ptr(weight), _ptr(out), dtype_code(out.dtype), out.stride(0),
           N, heads, dim, float(eps), _stream())
     return out
+
+
+# ---- keys and values in 8 bits, and copies of pages ------------------------------------------------------------------------
+def _on_current_device(*tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.is_cuda and t.device.index != _device():
+            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{_device()}")
+
+
+def _kv8_pages(pages: torch.Tensor, num_kv_heads: int, head_dim: int, page_size: int) -> None:
+    _need(num_kv_heads > 0 and page_size > 0 and 16 <= head_dim <= 256 and head_dim % 16 == 0,
+          "8-bit pages take head sizes that are multiples of 16 in 16..256, and at least one head and token")
+    _need(pages.dtype == torch.uint8 and pages.dim() == 2 and pages.is_contiguous() and pages.shape[0] > 0 and
+          pages.shape[1] == kv8_page_bytes(num_kv_heads, page_size, head_dim),
+          f"8-bit pages must be contiguous uint8 [pages, {kv8_page_bytes(num_kv_heads, page_size, head_dim)}] for {num_kv_heads} heads of "
+          f"{head_dim} and {page_size} tokens")
+
+
+def kv8_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor, num_kv_heads: int, head_dim: int,
+              page_size: int) -> None:
+    """Keys and values of rows ``k`` and ``v`` [tokens, kv heads * head_dim] (rows may lie apart) into the slots (page *
+    page_size + offset; negative: nowhere) of 8-bit pages (``cache.spec.KV8PagesSpec``). A page's rows in one call are
+    neighbours, in the order of the tokens (as a step's rows are). Each head's keys, and values, of a page share a scale, the
+    smallest power of two that holds them; storing behind a page's first token raises the scale where that is needed and
+    moves what the page holds up to there to it. A row at offset 0 starts its page anew. Infinities and NaN are held as NaN."""
+    _kv8_pages(pages, num_kv_heads, head_dim, page_size)
+    _i32(slots, "slots")
+    N = slots.numel()
+    _need(k.dim() == 2 and k.shape == (N, num_kv_heads * head_dim) and v.shape == k.shape and k.dtype == v.dtype,
+          "keys and values must be [tokens, kv heads * head_dim] of one type, one row per slot")
+    _need(N <= 1 or (k.stride(1) == 1 and v.stride(1) == 1), "the entries of a row of keys or values must be neighbours")
+    _on_current_device(k, v, slots, pages)
+    dtype = dtype_code(k.dtype)
+    _call("llmp_kv8_store", _ptr(k), k.stride(0), _ptr(v), v.stride(0), dtype, _ptr(slots), _ptr(pages), pages.shape[0], N,
+          num_kv_heads, head_dim, page_size, _stream())
+
+
+def kv8_gather(pages: torch.Tensor, block_tables: torch.Tensor, ctx_len: torch.Tensor, index: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """out[i] (``[n, 2, kv heads, page_size, head_dim]``, float32 or bfloat16, exact in either) = the values of the 8-bit page
+    that entry ``index[i]`` of the flattened ``block_tables`` names; zeros behind the request's last token and for a page that
+    is missing."""
+    _need(out.dim() == 5 and out.shape[1] == 2 and out.is_contiguous(), "unpacked pages must be contiguous [n, 2, kv heads, page_size, head_dim]")
+    nkv, page_size, d = out.shape[2:]
+    _kv8_pages(pages, nkv, d, page_size)
+    for name, t in (("block_tables", block_tables), ("ctx_len", ctx_len), ("index", index)):
+        _i32(t, name)
+    _need(block_tables.dim() == 2 and block_tables.shape[0] == ctx_len.numel(), "block tables must be [requests, pages]")
+    _need(index.numel() == out.shape[0], "one index per unpacked page")
+    _on_current_device(pages, block_tables, ctx_len, index, out)
+    dtype = dtype_code(out.dtype)
+    _call("llmp_kv8_gather", _ptr(pages), pages.shape[0], _ptr(block_tables), ctx_len.numel(), block_tables.shape[1], _ptr(ctx_len),
+          _ptr(index), index.numel(), _ptr(out), dtype, nkv, d, page_size, _stream())
+    return out
+
+
+def kv8_decode_scratch_floats(rows: int, num_heads: int, head_dim: int, max_ctx: int) -> int:
+    fn = library().llmp_kv8_decode_scratch_floats
+    fn.argtypes = [_I, _I, _I, _I]
+    fn.restype = _L
+    return int(fn(rows, num_heads, head_dim, max_ctx))
+
+
+def kv8_decode_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, pages: torch.Tensor, block_tables: torch.Tensor,
+                         ctx_len: torch.Tensor, max_ctx: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
+                         window: int, scale: float) -> torch.Tensor:
+    """Attention of one query row per request (row r belongs to request r, at position ctx_len[r] - 1) over the request's 8-bit
+    pages, as ``decode_attention`` over pages of q's type. No context is longer than ``max_ctx``. A request without keys gets zeros;
+    a page that is missing from the tables has no keys; what lies behind the context or before the window never matters."""
+    _kv8_pages(pages, num_kv_heads, head_dim, page_size)
+    _i32(block_tables, "block_tables")
+    _i32(ctx_len, "ctx_len")
+    R = ctx_len.numel()
+    _need(num_heads > 0 and num_heads % num_kv_heads == 0, f"{num_heads} query heads cannot share {num_kv_heads} key/value heads")
+    _need(q.dtype == out.dtype and q.dim() == 2 and q.shape[0] >= R and q.shape[1] >= num_heads * head_dim and q.stride(1) == 1 and
+          (R <= 1 or q.stride(0) == q_stride), "query rows must be [requests, at least heads * head_dim] of the output's type")
+    _need(out.is_contiguous() and out.shape == (R, num_heads * head_dim), "decode output must be [requests, heads * head_dim]")
+    _need(block_tables.dim() == 2 and block_tables.shape[0] == R and block_tables.shape[1] > 0, "block tables must be [requests, pages]")
+    _need(max_ctx > 0 and window >= 0, "the longest context must be positive, a window not negative")
+    _on_current_device(q, out, pages, block_tables, ctx_len)
+    dtype = dtype_code(q.dtype)
+    scratch = torch.empty(kv8_decode_scratch_floats(R, num_heads, head_dim, max_ctx), dtype=torch.float32, device=q.device)
+    _call("llmp_kv8_decode", _ptr(q), int(q_stride), _ptr(out), out.stride(0), dtype, _ptr(pages), pages.shape[0],
+          _ptr(block_tables), block_tables.shape[1], _ptr(ctx_len), R, int(max_ctx), num_heads, num_kv_heads, head_dim, page_size,
+          int(window), float(scale), _ptr(scratch), scratch.numel(), _stream())
+    return out
+
+
+def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
+    """tensor[dst[i]] = tensor[src[i]] for every i in each of the ``tensors`` (contiguous, one size of page, as many pages at
+    least as the numbers ask for), in one launch for as many as its parameters take. No destination may be a source or twice
+    a destination: the copies have no order."""
+    tensors, src, dst = list(tensors), [int(p) for p in src], [int(p) for p in dst]
+    _need(len(src) == len(dst), "as many destinations as sources are needed")
+    if not tensors or not src:
+        return
+    first = tensors[0]
+    _need(all(t.dim() >= 1 and t.is_contiguous() and t.dtype == first.dtype and t.shape[1:] == first.shape[1:] and t.device == first.device
+              for t in tensors), "the caches of a copy must be contiguous, of one page size, one type and on one device")
+    pages = min(t.shape[0] for t in tensors)
+    _need(all(0 <= p < pages for p in src) and all(0 <= p < pages for p in dst), f"a page to copy is outside 0..{pages - 1}")
+    _need(len(set(dst)) == len(dst) and not set(dst) & set(src), "a page is twice a destination, or a source and a destination")
+    _on_current_device(first)
+    page_bytes = first[0].numel() * first.element_size()
+    lib = library()
+    most_tensors, most_pairs = lib.llmp_copy_pages_max_tensors(), lib.llmp_copy_pages_max_pairs()
+    pointers = [_ptr(t) for t in tensors]
+    for at in range(0, len(pointers), most_tensors):
+        bases = (_P * len(pointers[at:at + most_tensors]))(*pointers[at:at + most_tensors])
+        for i in range(0, len(src), most_pairs):
+            n = len(src[i:i + most_pairs])
+            _call("llmp_copy_pages", bases, len(bases), page_bytes, (_I * n)(*src[i:i + n]), (_I * n)(*dst[i:i + n]), n, _stream())

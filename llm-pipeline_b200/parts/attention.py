@@ -23,8 +23,8 @@ from typing import Dict, List, Optional
 
 import torch
 
-from ..cache.spec import KVPagesSpec
-from ..ops import kernels
+from ..cache.spec import KV8PagesSpec, KVPagesSpec
+from ..ops import kernels, kv8
 from ..ops.linear import PendingProduct, linear, pending_product
 from ..weights.source import ParamSpec
 from .base import LayerCache, Mixer, TensorGetter
@@ -116,6 +116,9 @@ class PagedAttention(Mixer):
     def cache_spec(self) -> Optional[KVPagesSpec]:
         return KVPagesSpec(self.num_kv_heads, self.head_dim, self.window)
 
+    def cache_spec_8bit(self) -> Optional[KV8PagesSpec]:
+        return KV8PagesSpec(self.num_kv_heads, self.head_dim, self.window)
+
     # -- weights ---------------------------------------------------------------------------
     def _projections(self):
         return ("q_proj",) if self.kv_shared else ("q_proj", "k_proj", "v_proj")
@@ -160,7 +163,8 @@ class PagedAttention(Mixer):
     def forward_deferred(self, x, ctx, cache: LayerCache):
         if cache.pages is None or cache.group is None:
             raise RuntimeError("the attention mixer needs the pages of its cache")
-        page_size = cache.pages.shape[3]
+        eight = cache.pages.dtype == torch.uint8
+        page_size = cache.page_size if eight else cache.pages.shape[3]
         if self.tokens_per_tile is None:
             self.tokens_per_tile = kernels.tokens_per_attention_tile(self.num_heads, self.num_kv_heads, x.dtype,
                                                                      self.head_dim, page_size)
@@ -174,8 +178,11 @@ class PagedAttention(Mixer):
         kernels.qkv_post(qkv, self.num_heads, 0 if self.kv_shared else self.num_kv_heads, self.head_dim,
                          bias=self.b_qkv, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.qk_norm_eps,
                          cos=cos, sin=sin, rotary_dim=self.rotary_dim,
-                         slots=ctx.slot_mapping[cache.group] if writes else None,
-                         pages=cache.pages if writes else None, page_size=page_size)
+                         slots=ctx.slot_mapping[cache.group] if writes and not eight else None,
+                         pages=cache.pages if writes and not eight else None, page_size=page_size, keep_rows=writes and eight)
+        if writes and eight:
+            k, v = qkv[:, self.q_size:self.q_size + self.kv_size], qkv[:, self.q_size + self.kv_size:]
+            kernels.kv8_store(k, v, ctx.slot_mapping[cache.group], cache.pages, self.num_kv_heads, self.head_dim, page_size)
         out = torch.empty((ctx.num_tokens, self.q_size), dtype=x.dtype, device=x.device)
         self.attend(ctx, qkv, out, cache)
         return pending_product(out, self.w_o), self.b_o
@@ -212,6 +219,9 @@ class PagedAttention(Mixer):
     def attend(self, ctx, qkv: torch.Tensor, out: torch.Tensor, cache: LayerCache) -> None:
         """Causal attention of the step's query rows (the first ``num_heads * head_dim`` columns of ``qkv``) over the
         pages of ``cache``."""
+        if cache.pages.dtype == torch.uint8:
+            self.attend_8bit(ctx, qkv, out, cache)
+            return
         page_size = cache.pages.shape[3]
         tables = ctx.block_tables[cache.group]
         if ctx.max_q_len == 1:
@@ -234,3 +244,21 @@ class PagedAttention(Mixer):
         kernels.paged_attention(qkv, qkv.stride(0), out, cache.pages, tables, ctx.q_start, ctx.ctx_len, tile_req, tile_tok0,
                                 self.num_heads, self.num_kv_heads, self.head_dim, page_size, self.window or 0, self.scale,
                                 self.tokens_per_tile, tile_seg, tile_slot, places)
+
+    def attend_8bit(self, ctx, qkv: torch.Tensor, out: torch.Tensor, cache: LayerCache) -> None:
+        """The same over pages in 8 bits: single tokens read them as they are (those at the front of a mixed step too: their pages
+        then need not be unpacked), for prompt portions the pages of their requests are unpacked first."""
+        tables = ctx.block_tables[cache.group]
+        lead = ctx.num_requests if ctx.max_q_len == 1 else ctx.leading_single
+        if lead:
+            bound = (ctx.decode_ctx_bound or ctx.max_ctx_len) if ctx.max_q_len == 1 else ctx.leading_longest
+            kernels.kv8_decode_attention(qkv, qkv.stride(0), out[:lead], cache.pages, tables[:lead], ctx.ctx_len[:lead], bound, self.num_heads,
+                                         self.num_kv_heads, self.head_dim, cache.page_size, self.window or 0, self.scale)
+        if lead == ctx.num_requests:
+            return
+        key = ("kv8_prompts", self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size, self.window, lead)
+        plan = ctx.memo.get(key)
+        if plan is None:
+            plan = ctx.memo[key] = kv8.PromptPlan(ctx.starts, ctx.q_lens, self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size,
+                                                  self.window or 0, qkv.dtype, qkv.device, first_request=lead)
+        kv8.prompt_attention(plan, qkv, qkv.stride(0), out, cache.pages, tables, ctx.q_start, ctx.ctx_len, self.scale)

@@ -40,12 +40,14 @@ TensorGetter = Callable[[str, str], torch.Tensor]   # (full tensor name, role) -
 class LayerCache:
     """What one execution of a layer may touch: the pages of its cache id (``writes`` is False when
     an earlier execution owns them), the index of their group (for block tables and slot
-    mappings in the step context), and the state tensor ``[slots, ...]`` of its cache id."""
+    mappings in the step context), the state tensor ``[slots, ...]`` of its cache id, and the tokens of a page
+    (pages of bytes do not show it in their shape)."""
 
     pages: Optional[torch.Tensor] = None
     group: Optional[int] = None
     state: Optional[torch.Tensor] = None
     writes: bool = True
+    page_size: Optional[int] = None
 
 
 @dataclass
@@ -227,6 +229,11 @@ class PositionEncoding(Part):
 
 class Mixer(Part):
     def cache_spec(self) -> Optional[PagesSpec]:
+        return None
+
+    def cache_spec_8bit(self) -> Optional[PagesSpec]:
+        """What the mixer asks for where keys and values are to be held in 8 bits; None: it has no such form (and keeps
+        ``cache_spec``). The mixer sees which of the two it has got by its pages."""
         return None
 
     def state_spec(self) -> Optional[StateSpec]:

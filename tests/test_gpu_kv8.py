@@ -1,0 +1,429 @@
+"""Keys and values in 8 bits: storing, unpacking, attention of single tokens and of prompt portions, against plain forms in 64
+bits (``kv8_plain.py``)."""
+
+import math
+
+import pytest
+import torch
+
+import kv8_plain as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [pytest.param(torch.float32, id="f32"), pytest.param(torch.bfloat16, id="bf16")]
+SIZES = [(32, 8, 128, 16), (16, 8, 128, 8), (64, 8, 128, 32), (9, 1, 128, 64), (6, 2, 80, 8), (5, 5, 48, 4), (12, 1, 256, 16), (40, 2, 128, 16),
+         (4, 4, 16, 1), (2, 1, 128, 128), (8, 4, 64, 24)]
+
+
+def K():
+    from llm_pipeline_b200.ops import kernels
+    return kernels
+
+
+def same_bytes(got, want, where=""):
+    got, want = got.cpu(), want.cpu()
+    assert got.shape == want.shape
+    bad = (got != want).nonzero()
+    assert bad.numel() == 0, f"{where}: {bad.shape[0]} bytes differ, the first at {bad[0].tolist()}: {got[tuple(bad[0])]} and not {want[tuple(bad[0])]}"
+
+
+def filled(P, nkv, ps, d, seed, wild=True):
+    """Host pages with scales of their own in every block, as bytes."""
+    gen = torch.Generator().manual_seed(seed)
+    host = plain.Pages(P, nkv, ps, d)
+    host.q.copy_(torch.randint(0, 256, host.q.shape, generator=gen, dtype=torch.int32).to(torch.uint8))
+    host.q[(host.q & 127) == 127] -= 1                                           # numbers alone
+    host.e.copy_((torch.randint(117, 123, host.e.shape, generator=gen) if wild else torch.full(host.e.shape, 119)).to(torch.uint8))
+    return host
+
+
+# ---- storing and unpacking -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,ps", SIZES)
+def test_store_matches_the_plain_form_to_the_bit(dtype, nq, nkv, d, ps):
+    """Three calls one after another: rows at the start of pages, in their middle, over several pages, one by one; rows of very
+    different sizes, so that scales rise; rows of a strided matrix."""
+    gen = torch.Generator().manual_seed(ps * d + nkv)
+    P = 9
+    host = filled(P, nkv, ps, d, 1)
+    pages = host.raw.to(DEV)
+    steps = [list(range(3 * ps, 3 * ps + 2 * ps + ps // 2 + 1)) + [7 * ps],                    # two pages and a part, another request's first token
+             [7 * ps + 1] if ps > 1 else [8 * ps],
+             list(range(5 * ps + ps // 2 + 1, 6 * ps)) + list(range(1 * ps, 2 * ps)) + [-1] + [2 * ps + ps // 3]]
+    for n, slots in enumerate(steps):
+        N = len(slots)
+        qkv = torch.randn(N, (nq + 2 * nkv) * d, generator=gen) * torch.exp(2.0 * torch.randn(N, 1, generator=gen)) * 10.0 ** n
+        qkv = qkv.to(dtype)
+        k, v = qkv[:, nq * d:(nq + nkv) * d], qkv[:, (nq + nkv) * d:]
+        host.store(k, v, slots)
+        on = qkv.to(DEV)
+        K().kv8_store(on[:, nq * d:(nq + nkv) * d], on[:, (nq + nkv) * d:], torch.tensor(slots, dtype=torch.int32, device=DEV), pages, nkv, d, ps)
+        same_bytes(pages, host.raw, f"step {n}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_store_of_unusual_numbers(dtype):
+    """Zeros, the largest and the smallest numbers, infinities and NaN, a page that only gets zeros, a duplicate slot, slots beyond the
+    pages, values on the border between two scales and on ties."""
+    nkv, d, ps = 2, 32, 8
+    host = filled(4, nkv, ps, d, 2)
+    pages = host.raw.to(DEV)
+    top = torch.finfo(dtype).max
+    rows = torch.zeros(14, 2 * nkv * d)
+    rows[1, :] = 448.0
+    rows[1, 3] = -448.0
+    rows[2, ::2] = 450.0
+    rows[3, 5] = math.inf
+    rows[3, 6] = -math.inf
+    rows[3, 7] = math.nan
+    rows[3, 40] = 1e-3
+    rows[4, :] = top
+    rows[5, :] = torch.finfo(dtype).tiny
+    rows[6, ::3] = torch.finfo(dtype).tiny / 64
+    rows[7, :] = torch.linspace(-20, 20, 2 * nkv * d)
+    rows[8, :] = (torch.arange(2 * nkv * d) % 33) / 16.0 + 1.0                   # halves between steps: ties
+    rows[9, :] = math.nan
+    rows[10, :] = math.inf
+    rows[11, :] = -0.0
+    rows[12, :] = 2.0 ** -9 * 1.5
+    rows[12, 0] = 448.0
+    rows[13, :] = 5.0
+    rows = rows.to(dtype)
+    for slots in ([0, 1, 2, 3, 4], [8, 9, 10, 11, 12, 13, 14], [16, 17], [24, 25, 26, 27, 28]):
+        first = {0: 0, 8: 5, 16: 9, 24: 9}[slots[0]]
+        part = rows[first:first + len(slots)]
+        k, v = part[:, :nkv * d], part[:, nkv * d:]
+        host.store(k, v, slots)
+        on = part.to(DEV)
+        K().kv8_store(on[:, :nkv * d], on[:, nkv * d:], torch.tensor(slots, dtype=torch.int32, device=DEV), pages, nkv, d, ps)
+        same_bytes(pages, host.raw, str(slots))
+    # the same slot twice (the later row stays), rows without a slot inside a run, slots beyond the pages
+    slots = [16, -1, 17, 18, 18, 32, 19, 1 << 30]
+    part = rows[4:12]
+    k, v = part[:, :nkv * d], part[:, nkv * d:]
+    host.store(k, v, slots)
+    on = part.to(DEV)
+    K().kv8_store(on[:, :nkv * d], on[:, nkv * d:], torch.tensor(slots, dtype=torch.int32, device=DEV), pages, nkv, d, ps)
+    same_bytes(pages, host.raw, "twice")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_store_cut_into_any_steps_holds_the_same_but_for_the_smallest_values(dtype):
+    """A prompt in one call, in portions and token by token: the same scales, and values that differ by at most one rounding
+    below the new scale's normal numbers (half of 2^-9)."""
+    nkv, d, ps, N = 2, 64, 16, 41
+    gen = torch.Generator().manual_seed(3)
+    x = (torch.randn(N, 2 * nkv * d, generator=gen) * torch.exp(1.5 * torch.randn(N, 1, generator=gen))).to(dtype).to(DEV)
+    got = []
+    for cut in ([N], [5, 16, 16, 4], [1] * N):
+        pages = torch.zeros(3, plain.page_bytes(nkv, ps, d), dtype=torch.uint8, device=DEV)
+        at = 0
+        for n in cut:
+            part = x[at:at + n]
+            K().kv8_store(part[:, :nkv * d], part[:, nkv * d:], torch.arange(at, at + n, dtype=torch.int32, device=DEV), pages, nkv, d, ps)
+            at += n
+        got.append(plain.Pages(3, nkv, ps, d, pages))
+    whole = got[0]
+    for other in got[1:]:
+        assert torch.equal(whole.e, other.e)
+        far = (whole.values([0, 1, 2]) - other.values([0, 1, 2])).abs()
+        assert bool((far <= 2.0 ** -9 * plain.power(whole.e.int() - 127)[..., None, None]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nkv,d,ps", [(8, 128, 16), (1, 16, 1), (3, 80, 24), (2, 256, 128)])
+def test_gather_is_exact_and_zeros_what_is_not_there(dtype, nkv, d, ps):
+    P = 7
+    host = filled(P, nkv, ps, d, 5)
+    host.q[3, :, :, ps // 2 + 1:] = 127                                          # NaN behind the end of request 0
+    tables = torch.tensor([[5, 3, 2], [1, -1, 99]], dtype=torch.int32)
+    ctx = [ps + ps // 2 + 1, 3 * ps]
+    index = [1, 0, 3, 4, 5, 2, 17, -1]
+    want = torch.zeros(len(index), 2, nkv, ps, d, dtype=torch.float64)
+    for i, entry in enumerate(index):
+        if not 0 <= entry < 6 or not 0 <= int(tables.flatten()[entry]) < P:
+            continue
+        there = ctx[entry // 3] - entry % 3 * ps
+        if there > 0:
+            want[i, :, :, :there] = host.values([int(tables.flatten()[entry])])[0][:, :, :there]
+    out = torch.full((len(index), 2, nkv, ps, d), 7.0, dtype=dtype, device=DEV)
+    K().kv8_gather(host.raw.to(DEV), tables.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV),
+                   torch.tensor(index, dtype=torch.int32, device=DEV), out)
+    assert torch.equal(out.double().cpu(), want)
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------
+
+def scattered(ctx, ps, P, seed):
+    """Block tables of requests of ``ctx`` tokens over shuffled pages; one entry more than the longest needs, -1 where there is none."""
+    gen = torch.Generator().manual_seed(seed)
+    ids = torch.randperm(P, generator=gen).tolist()
+    width = max(1, max(-(-c // ps) for c in ctx)) + 1
+    tables = torch.full((len(ctx), width), -1, dtype=torch.int32)
+    for r, c in enumerate(ctx):
+        for j in range(-(-c // ps)):
+            tables[r, j] = ids.pop()
+    return tables
+
+
+def spoil(host, tables, ctx, ps):
+    """NaN in every slot behind the contexts and in every page that no table names."""
+    named = set(int(p) for p in tables.flatten() if p >= 0)
+    for p in range(host.q.shape[0]):
+        if p not in named:
+            host.q[p] = 127
+            host.e[p] = 255
+    for r, c in enumerate(ctx):
+        if c % ps:
+            host.q[int(tables[r, c // ps]), :, :, c % ps:] = 127
+
+
+def bound(out, size, top, dtype, d):
+    """How far a row may be off. The result is rounded once. In bfloat16 the weights are rounded to half precision at best, to 2^-11
+    of themselves on either side, and their sum is not: 2^-10 of sum w |v| takes both. In either type a score of d products of
+    magnitude sum |q||k| scale = top is off by at most (d + 4) 2^-24 top, which moves weights by that much, twice (weight and sum);
+    sums of weights and values in tiles, splits and warps add 2^-24 for every of at most 64 terms in a row of additions."""
+    half = torch.finfo(dtype).eps / 2
+    weights = 2.0 ** -10 if dtype == torch.bfloat16 else 0.0
+    return half * out.abs() + size * (weights + 2 * (d + 4) * 2.0 ** -24 * top + 128 * 2.0 ** -24) + 1e-30
+
+
+CONTEXTS = {"short": [1, 0, 15, 16, 17, 2], "mixed": [129, 700, 1, 256, 31, 64, 333], "long": [2100, 5, 1024, 1500]}
+
+
+def decode_case(nq, nkv, d, ps, ctx, dtype, seed, wild=True):
+    gen = torch.Generator().manual_seed(seed)
+    P = sum(-(-c // ps) for c in ctx) + 3
+    host = filled(P, nkv, ps, d, seed, wild)
+    tables = scattered(ctx, ps, P, seed)
+    q = torch.randn(len(ctx), nq * d + 32, generator=gen).to(dtype)
+    return host, tables, q
+
+
+def check_decode(host, tables, q, ctx, nq, nkv, d, ps, window, dtype, out, scale):
+    for r, c in enumerate(ctx):
+        k, v, there = host.request(tables[r], c)
+        want, size, top = plain.attend(q[r:r + 1, :nq * d].view(1, nq, d), k, v, [c - 1], there, scale, window)
+        got = out[r].double().cpu().view(1, nq, d)
+        far = (got - want).abs()
+        allowed = bound(want, size, top, dtype, d)
+        assert bool((far <= allowed).all()), f"request {r} of {c} keys: {float((far / allowed).max())} times what it may be off"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("lengths", sorted(CONTEXTS))
+@pytest.mark.parametrize("nq,nkv,d,ps", SIZES)
+def test_single_tokens(dtype, nq, nkv, d, ps, lengths, window):
+    ctx = CONTEXTS[lengths]
+    host, tables, q = decode_case(nq, nkv, d, ps, ctx, dtype, len(ctx) + d)
+    spoil(host, tables, ctx, ps)
+    if window:                                                                   # pages that have left the window are gone
+        for r, c in enumerate(ctx):
+            tables[r, :max(0, c - window) // ps] = -1
+    out = torch.full((len(ctx), nq * d), 9.0, dtype=dtype, device=DEV)
+    K().kv8_decode_attention(q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV),
+                             max(ctx) + 100, nq, nkv, d, ps, window, d ** -0.5)
+    check_decode(host, tables, q, ctx, nq, nkv, d, ps, window, dtype, out, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,ps", [(32, 8, 128, 16), (6, 2, 80, 8)])
+def test_single_tokens_over_blocks_of_very_different_scales(dtype, nq, nkv, d, ps):
+    """Value blocks from 2^-60 to 2^60, blocks of zeros whose scale byte is 0 among them: every key has its weight, whatever its
+    value's scale; a page missing in the middle has no keys."""
+    ctx = [300, 64, 17]
+    host, tables, q = decode_case(nq, nkv, d, ps, ctx, dtype, 11)
+    gen = torch.Generator().manual_seed(4)
+    host.e[:, 1] = torch.randint(67, 188, host.e[:, 1].shape, generator=gen).to(torch.uint8)
+    empty = torch.rand(host.e[:, 1].shape, generator=gen) < 0.3
+    host.e[:, 1][empty] = 0
+    host.q[:, 1][empty] = 0
+    tables[0, 3] = -1
+    tables[1, 1] = 1000
+    out = torch.empty((len(ctx), nq * d), dtype=dtype, device=DEV)
+    K().kv8_decode_attention(q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV),
+                             max(ctx), nq, nkv, d, ps, 0, d ** -0.5)
+    check_decode(host, tables, q, ctx, nq, nkv, d, ps, 0, dtype, out, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,ps", [(32, 8, 128, 16), (6, 2, 80, 8)])
+def test_single_tokens_with_sharp_and_flat_scores(dtype, nq, nkv, d, ps):
+    """Queries of very different sizes in one group: weights from one-hot to even; a query of zeros; what is no number in a query or
+    in a seen key makes its rows no number and no others."""
+    ctx = [200, 90]
+    host, tables, q = decode_case(nq, nkv, d, ps, ctx, torch.float32, 12, wild=False)
+    q[:, :nq * d].view(2, nq, d).mul_(torch.logspace(-6, 0.6, nq)[None, :, None])
+    q[0, :d] = 0
+    q = q.to(dtype)
+    out = torch.empty((len(ctx), nq * d), dtype=dtype, device=DEV)
+    call = lambda pages, qq: K().kv8_decode_attention(qq.to(DEV), q.stride(0), out, pages.to(DEV), tables.to(DEV),      # noqa: E731
+                                                      torch.tensor(ctx, dtype=torch.int32, device=DEV), max(ctx), nq, nkv, d, ps, 0, 1.0)
+    call(host.raw, q)
+    check_decode(host, tables, q, ctx, nq, nkv, d, ps, 0, dtype, out, 1.0)
+    clean = out.clone()
+    host.q[int(tables[0, 1]), 0, 0, 0, 5] = 127                                  # one key of head 0 of request 0
+    bad = q.clone()
+    bad[1, d + 3] = math.nan
+    call(host.raw, bad)
+    nan = out.view(2, nq, d).isnan()
+    G = nq // nkv
+    assert bool(nan[0, :G].all()) and not bool(nan[0, G:].any())
+    assert bool(nan[1, 1].all()) and int(nan[1].sum()) == d
+    assert torch.equal(out.view(2, nq, d)[~nan], clean.view(2, nq, d)[~nan])
+
+
+def test_single_tokens_in_a_page_pool_beyond_four_gigabytes():
+    """Pages whose bytes begin beyond 32-bit offsets."""
+    nq, nkv, d, ps = 32, 8, 128, 64
+    size = plain.page_bytes(nkv, ps, d)
+    P = (1 << 32) // size + 9
+    pages = torch.zeros(P, size, dtype=torch.uint8, device=DEV)
+    ctx = [150]
+    host, _t, q = decode_case(nq, nkv, d, ps, ctx, torch.bfloat16, 21)
+    last = [P - 1, P - 3, P - 2]
+    pages[last] = host.raw[:3].to(DEV)
+    tables = torch.tensor([last], dtype=torch.int32)
+    x = torch.randn(1, 2 * nkv * d, generator=torch.Generator().manual_seed(1)).bfloat16()
+    K().kv8_store(x[:, :nkv * d].to(DEV), x[:, nkv * d:].to(DEV), torch.tensor([(P - 2) * ps + 21], dtype=torch.int32, device=DEV), pages, nkv, d, ps)
+    host.store(x[:, :nkv * d], x[:, nkv * d:], [2 * ps + 21])
+    same_bytes(pages[last], host.raw[:3])
+    out = torch.empty(1, nq * d, dtype=torch.bfloat16, device=DEV)
+    K().kv8_decode_attention(q.to(DEV), q.stride(0), out, pages, tables.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV), 150, nq, nkv, d, ps,
+                             0, d ** -0.5)
+    check_decode(host, torch.tensor([[0, 1, 2]]), q, ctx, nq, nkv, d, ps, 0, torch.bfloat16, out, d ** -0.5)
+
+
+def prompt(case, starts, lens, window, dtype, seed, first=0):
+    from llm_pipeline_b200.ops import kv8
+
+    nq, nkv, d, ps = case
+    ctx = [s + n for s, n in zip(starts, lens)]
+    P = sum(-(-c // ps) for c in ctx) + 3
+    host = filled(P, nkv, ps, d, seed)
+    tables = scattered(ctx, ps, P, seed)
+    spoil(host, tables, ctx, ps)
+    N = sum(lens)
+    q = torch.randn(N + 2, (nq + 2 * nkv) * d, generator=torch.Generator().manual_seed(seed)).to(dtype)
+    out = torch.full((N + 2, nq * d), 9.0, dtype=dtype, device=DEV)
+    plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, window, dtype, torch.device(DEV), first_request=first)
+    dev = dict(pages=host.raw.to(DEV), tables=tables.to(DEV), ctx=torch.tensor(ctx, dtype=torch.int32, device=DEV), q=q.to(DEV),
+               start=torch.tensor([sum(lens[:r]) for r in range(len(lens) + 1)], dtype=torch.int32, device=DEV))
+    kv8.prompt_attention(plan, dev["q"], q.stride(0), out, dev["pages"], dev["tables"], dev["start"], dev["ctx"], d ** -0.5)
+    return host, tables, ctx, q, out
+
+
+PORTIONS = [([0], [1]), ([0], [300]), ([37, 0, 500], [129, 1, 70]), ([1000, 3], [2, 40])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("portions", range(len(PORTIONS)))
+@pytest.mark.parametrize("nq,nkv,d,ps", [(32, 8, 128, 16), (6, 2, 80, 8), (5, 5, 48, 4), (9, 1, 128, 64)])
+def test_prompt_portions(dtype, nq, nkv, d, ps, portions, window):
+    starts, lens = PORTIONS[portions]
+    host, tables, ctx, q, out = prompt((nq, nkv, d, ps), starts, lens, window, dtype, 31 + portions)
+    at = 0
+    for r, n in enumerate(lens):
+        rows = sorted({0, 1, n // 2, n - 1} & set(range(n)))
+        k, v, there = host.request(tables[r], ctx[r])
+        want, size, top = plain.attend(q[[at + i for i in rows], :nq * d].view(-1, nq, d), k, v, [starts[r] + i for i in rows], there, d ** -0.5, window)
+        far = (out[[at + i for i in rows]].double().cpu().view(-1, nq, d) - want).abs()
+        # the kernel over unpacked pages rounds the weights to bfloat16 (2^-8 of themselves, and their sum is not rounded)
+        allowed = bound(want, size, top, dtype, d) + (2.0 ** -8 * size if dtype == torch.bfloat16 else 0)
+        assert bool((far <= allowed).all()), f"request {r}: {float((far / allowed).max())}"
+        at += n
+    assert bool((out[at:] == 9).all())                                           # rows behind the last request's
+
+
+def test_prompt_portions_in_turns_of_a_small_workspace(monkeypatch):
+    from llm_pipeline_b200.ops import kv8
+
+    case, starts, lens = (32, 8, 128, 16), [37, 0, 500, 20], [129, 1, 70, 33]
+    whole = prompt(case, starts, lens, 0, torch.bfloat16, 41)[-1]
+    monkeypatch.setattr(kv8, "WORKSPACE_BYTES", 1 << 20)
+    assert torch.equal(prompt(case, starts, lens, 0, torch.bfloat16, 41)[-1], whole)
+    # the first requests left to another kernel
+    part = prompt(case, starts, lens, 0, torch.bfloat16, 41, first=2)[-1]
+    assert bool((part[:130] == 9).all()) and torch.equal(part[130:], whole[130:])
+
+
+def test_a_step_in_a_graph_and_on_two_streams():
+    """Store and attention captured, replayed over other contents; two such calls at once on two streams."""
+    nq, nkv, d, ps = 32, 8, 128, 16
+    ctx = [333, 40, 1000]
+    sets = []
+    for seed in (51, 52):
+        host, tables, q = decode_case(nq, nkv, d, ps, ctx, torch.bfloat16, seed)
+        x = torch.randn(3, 2 * nkv * d, generator=torch.Generator().manual_seed(seed)).bfloat16()
+        slots = [int(tables[r, (c - 1) // ps]) * ps + (c - 1) % ps for r, c in enumerate(ctx)]
+        sets.append((host, tables, q, x, slots))
+    dev = [[host.raw.to(DEV), tables.to(DEV), q.to(DEV), x.to(DEV), torch.tensor(slots, dtype=torch.int32, device=DEV),
+            torch.tensor(ctx, dtype=torch.int32, device=DEV), torch.empty(3, nq * d, dtype=torch.bfloat16, device=DEV)]
+           for host, tables, q, x, slots in sets]
+
+    def call(t):
+        pages, tables, q, x, slots, n, out = t
+        K().kv8_store(x[:, :nkv * d], x[:, nkv * d:], slots, pages, nkv, d, ps)
+        K().kv8_decode_attention(q, q.stride(0), out, pages, tables, n, 1024, nq, nkv, d, ps, 0, d ** -0.5)
+
+    fresh = [t[0].clone() for t in dev]
+    call(dev[0])
+    graphs = []
+    for t in dev:
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(t)
+        graphs.append(g)
+    for host, tables, q, x, slots in sets:
+        host.store(x[:, :nkv * d], x[:, nkv * d:], slots)
+    for how in ("graphs", "streams"):
+        for t, raw in zip(dev, fresh):
+            t[0].copy_(raw)
+            t[-1].zero_()
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for _ in range(20):
+            for t, g, s in zip(dev, graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay() if how == "graphs" else call(t)
+        torch.cuda.synchronize()
+        for t, (host, tables, q, x, slots) in zip(dev, sets):
+            same_bytes(t[0], host.raw, how)
+            check_decode(host, tables, q, ctx, nq, nkv, d, ps, 0, torch.bfloat16, t[-1], d ** -0.5)
+
+
+def test_empty_calls_do_nothing():
+    nkv, d, ps = 2, 32, 8
+    pages = torch.full((2, plain.page_bytes(nkv, ps, d)), 3, dtype=torch.uint8, device=DEV)
+    none = torch.empty(0, nkv * d, device=DEV)
+    i32 = lambda *s: torch.empty(*s, dtype=torch.int32, device=DEV)             # noqa: E731
+    K().kv8_store(none, none, i32(0), pages, nkv, d, ps)
+    K().kv8_gather(pages, i32(0, 3), i32(0), i32(0), torch.empty(0, 2, nkv, ps, d, device=DEV))
+    K().kv8_decode_attention(torch.empty(0, 4 * d, device=DEV), 4 * d, torch.empty(0, 4 * d, device=DEV), pages, i32(0, 3), i32(0), 5, 4, nkv, d, ps, 0, 1.0)
+    assert bool((pages == 3).all())
+
+
+# ---- copies ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape,dtype", [((2, 8, 16, 128), torch.bfloat16), ((33024,), torch.uint8), ((7,), torch.uint8), ((5, 3), torch.float32)])
+@pytest.mark.parametrize("tensors,pairs", [(1, 1), (50, 3), (2, 900)])
+def test_copy_pages(shape, dtype, tensors, pairs):
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    P = 2 * pairs + 3
+    if tensors * P * math.prod(shape) > 1 << 28:
+        tensors = 1
+    caches = [torch.randint(0, 200, (P,) + shape, generator=gen, device=DEV).to(dtype) for _ in range(tensors)]
+    order = torch.randperm(P, generator=torch.Generator().manual_seed(6)).tolist()
+    src, dst = order[:pairs], order[pairs:2 * pairs]
+    if pairs > 1:
+        src[1] = src[0]                                                          # one page to two places
+    want = [t.clone() for t in caches]
+    for t in want:
+        t[dst] = t[src]
+    K().copy_pages(caches, src, dst)
+    for got, t in zip(caches, want):
+        assert torch.equal(got, t)
