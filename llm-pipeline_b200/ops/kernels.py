@@ -9,6 +9,7 @@ tensor that is not on a CUDA device is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional, Sequence, Tuple
 
@@ -122,6 +123,7 @@ _SIGNATURES = {
     "llmp_kv8_store": [_P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _I, _P],
     "llmp_kv8_gather": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P],
     "llmp_kv8_decode": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
+    "llmp_kv8_stream": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P, _P],
     "llmp_copy_pages": [_P, _I, _L, _P, _P, _I, _P],
 }
 _bound = {}
@@ -2360,6 +2362,37 @@ def kv8_decode_scratch_floats(rows: int, num_heads: int, head_dim: int, max_ctx:
     return int(fn(rows, num_heads, head_dim, max_ctx))
 
 
+@functools.lru_cache(maxsize=None)
+def kv8_stream_supports(dtype: torch.dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
+    """Whether single tokens over 8-bit pages of these sizes get the streaming kernel (query rows that start on 16 bytes)."""
+    return dtype == torch.bfloat16 and bool(library().llmp_kv8_stream_supports(num_heads, num_kv_heads, head_dim, page_size))
+
+
+_kv8_sizes: Optional[Tuple[int, int]] = None     # floats of scratch and counters of a launch of the streaming kernel
+_kv8_counters: dict = {}
+KV8_CAPTURED_CALLS = 4096                        # captured calls with counters from the slab
+
+
+def kv8_counters(device: torch.device, count: int) -> torch.Tensor:
+    """Zeroed counters for a launch of the streaming kernel, which leaves them zero. Calls on one stream follow one another
+    and share a set. A captured call gets a set of its own, since its graph may be replayed beside others: from a slab that was
+    made outside a capture, or, where there is none or it is used up, zeroed by the graph itself."""
+    key = device.index
+    if torch.cuda.is_current_stream_capturing():
+        slab = _kv8_counters.get((key, "slab"))
+        if slab is None or slab[1] + count > slab[0].numel():
+            return torch.zeros(count, dtype=torch.int32, device=device)
+        slab[1] += count
+        return slab[0][slab[1] - count:slab[1]]
+    counters = _kv8_counters.get((key, _stream()))
+    if counters is None:
+        counters = _kv8_counters[key, _stream()] = torch.zeros(count, dtype=torch.int32, device=device)
+        if (key, "slab") not in _kv8_counters:
+            _kv8_counters[key, "slab"] = [torch.zeros(KV8_CAPTURED_CALLS * count, dtype=torch.int32, device=device), 0]
+            torch.cuda.current_stream(device).synchronize()      # its captured users are ordered by nothing else
+    return counters
+
+
 def kv8_decode_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, pages: torch.Tensor, block_tables: torch.Tensor,
                          ctx_len: torch.Tensor, max_ctx: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                          window: int, scale: float) -> torch.Tensor:
@@ -2378,6 +2411,17 @@ def kv8_decode_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
     _need(max_ctx > 0 and window >= 0, "the longest context must be positive, a window not negative")
     _on_current_device(q, out, pages, block_tables, ctx_len)
     dtype = dtype_code(q.dtype)
+    if kv8_stream_supports(q.dtype, num_heads, num_kv_heads, head_dim, page_size) and (q.data_ptr() | 2 * int(q_stride)) % 16 == 0:
+        global _kv8_sizes
+        if _kv8_sizes is None:
+            fn = library().llmp_kv8_stream_scratch_floats
+            fn.restype = _L
+            _kv8_sizes = int(fn()), int(library().llmp_kv8_stream_counters())
+        scratch = torch.empty(_kv8_sizes[0], dtype=torch.float32, device=q.device)
+        _call("llmp_kv8_stream", _ptr(q), int(q_stride), _ptr(out), out.stride(0), _ptr(pages), pages.shape[0], _ptr(block_tables),
+              block_tables.shape[1], _ptr(ctx_len), R, int(max_ctx), num_heads, num_kv_heads, page_size, int(window), float(scale), _ptr(scratch),
+              _kv8_sizes[0], _ptr(kv8_counters(q.device, _kv8_sizes[1])), error_flag().data_ptr(), _stream())
+        return out
     scratch = torch.empty(kv8_decode_scratch_floats(R, num_heads, head_dim, max_ctx), dtype=torch.float32, device=q.device)
     _call("llmp_kv8_decode", _ptr(q), int(q_stride), _ptr(out), out.stride(0), dtype, _ptr(pages), pages.shape[0],
           _ptr(block_tables), block_tables.shape[1], _ptr(ctx_len), R, int(max_ctx), num_heads, num_kv_heads, head_dim, page_size,

@@ -90,6 +90,16 @@ class Pages:
         scale = torch.where(e > 0, power(e - 127), torch.zeros(e.shape, dtype=torch.float64))
         return E4M3[self.q[ids].long()] * scale[..., None, None]
 
+    def value_scales(self, table, ctx):
+        """[ctx, nkv]: what the bytes of a request's values are to be multiplied by (1 for blocks of zeros and missing pages)."""
+        P, nkv, ps, d = self.sizes
+        ids = [int(p) if 0 <= int(p) < P else -1 for p in table[:-(-ctx // ps)]]
+        if not ids:
+            return torch.zeros(0, nkv, dtype=torch.float64)
+        e = self.e[[max(i, 0) for i in ids], 1].int()
+        e = torch.where((e > 0) & (torch.tensor(ids)[:, None] >= 0), e, torch.full_like(e, 127))
+        return power(e - 127).repeat_interleave(ps, 0)[:ctx]
+
     def request(self, table, ctx):
         """Keys and values [ctx, nkv, d] of a request and which of its keys are there (a page may be missing)."""
         P, nkv, ps, d = self.sizes
@@ -98,6 +108,22 @@ class Pages:
         held = self.values([p if 0 <= p < P else 0 for p in table]) if table else torch.zeros(0, 2, nkv, ps, d, dtype=torch.float64)
         k, v = held.permute(1, 0, 3, 2, 4).reshape(2, -1, nkv, d)[:, :ctx].unbind(0)
         return k, v, there
+
+
+def smallest(q, k, v, v_scales, position, there, scale, window):
+    """[nq, d]: 2^-25 max_j(w_j s_j) sum_j |b_j| of one row, with v_j = s_j b_j: what weights times the values' scales may be off by where
+    they are held in half precision relative to the largest of them (numbers below 2^-14 are 2^-24 apart)."""
+    nq, d = q.shape
+    T, nkv, _ = k.shape
+    j = torch.arange(T)
+    seen = there & (j <= position) & ((j > position - window) if window else (j >= 0))
+    if not bool(seen.any()):
+        return torch.zeros(nq, d, dtype=torch.float64)
+    G = nq // nkv
+    kk, s = k[seen].repeat_interleave(G, 1), v_scales[seen].repeat_interleave(G, 1)
+    w = torch.softmax(torch.einsum("hd,thd->ht", q.double().cpu(), kk) * scale, -1)
+    b = (v[seen] / v_scales[seen][..., None]).abs().sum(0).repeat_interleave(G, 0)
+    return 2.0 ** -25 * (w * s.t()).amax(-1, keepdim=True) * b
 
 
 def attend(q, k, v, positions, there, scale, window):
