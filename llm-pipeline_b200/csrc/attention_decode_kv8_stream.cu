@@ -1,5 +1,5 @@
 // Attention of single tokens over pages of 8-bit keys and values (kv8.cuh), bfloat16 queries, head size 128: one stream per
-// SM. A load warp keeps a ring of TMA boxes in flight, eight warps work through what has landed with mma.sync.
+// SM. Four warps keep a ring of TMA boxes in flight, eight work through what has landed with mma.sync.
 //
 // A row group is a request, a key/value head and up to eight of the query heads that share it. Its keys are cut into units of
 // 32 keys aligned to key 0 (8 KB: keys and values). The units of all row groups of the launch form one list, request by request,
@@ -21,8 +21,8 @@
 // when it is passed by 8) both keep their bits whatever the scales of the blocks are. out = O / l * 2^(mu - m).
 //
 // At the end of a segment (what a block has of a group) the warps' sums are added in shared memory. A whole group is written out;
-// of a shared one every block leaves its sums in global memory and counts itself, and the block that counts last adds them in block
-// order, writes, and sets the counter back to zero. Nobody waits for anybody. Every wait on an mbarrier is bounded: when one runs
+// of a shared one every block leaves its sums in global memory and counts itself at its end, and the block that counts last adds them
+// in block order, writes, and sets the counter back to zero. Nobody waits for anybody. Every wait on an mbarrier is bounded: when one runs
 // out the kernel records 1 in *error_flag and goes on without waiting (its output is then wrong; the host reads the flag).
 #include "kv8.cuh"
 #include "tcgen05.cuh"
@@ -31,15 +31,22 @@
 #define S8_WARPS 8
 #define S8_KEYS 32
 #define S8_STAGE_BYTES (2 * S8_KEYS * S8_D)
-#define S8_STAGES 20
-#define S8_THREADS ((S8_WARPS + 1) * 32)
+#define S8_DEPTH 2                                   // units of a warp in shared memory: the one it works on and the next
+#define S8_LOADERS 4                                 // warps that load
+#define S8_ASK 2                                     // units of a turn of theirs
+#define S8_THREADS ((S8_WARPS + S8_LOADERS) * 32)
 #define S8_HEADS 8
 #define S8_OSTRIDE (S8_D + 4)                        // floats of a row of a warp's sums in shared memory
 #define S8_MAX_ROWS 512
 #define S8_MAX_BLOCKS 256
-#define S8_GROUP_COST 4
+#define S8_GROUP_COST 16
 #define S8_MIN_SHARE 12
-#define S8_PART (S8_HEADS * S8_D + 3 * S8_HEADS)     // floats of a segment's sums: O, m, mu, l
+#define S8_OWN_UNITS 16                              // units of a block at least where a group has blocks of its own
+#define S8_EVEN_COST 16                              // what borders inside groups cost a block, in units
+// Unit n of a block lies in stage n mod (S8_WARPS S8_DEPTH) and is read by warp n mod S8_WARPS: a stage is always the same warp's. Boxes
+// do not land in the order in which they were asked for: were a stage read by two warps in turn, the second could look at its barrier while
+// the first's data is still on its way, one phase early, where a wait for a parity cannot tell that from one phase late.
+#define S8_PART (S8_HEADS * S8_D + 4 * S8_HEADS)     // floats of a segment's sums: O, then m, mu, l of each row
 
 struct Stream8Params {
     const bf16* q;
@@ -48,7 +55,7 @@ struct Stream8Params {
     const int* block_tables;
     const int* ctx_len;
     long q_stride, out_stride, page_bytes;
-    int table_stride, num_pages, max_ctx, R, nq, nkv, page_size, box_tokens, window;
+    int table_stride, num_pages, max_ctx, R, nq, nkv, page_size, page_shift, window;
     float scale;
     float* partials;                                 // [blocks][2][S8_PART]: the segment that began earlier, the one that goes on later
     unsigned* arrivals;                              // [blocks], zero between launches
@@ -152,33 +159,34 @@ struct Sums8 {
 
 __device__ __forceinline__ float s8_finite(float m) { return m == -INFINITY ? 0.f : m; }
 
-// One unit: `valid` has a bit for every key that counts (not 0), `meta` the scale bytes of its four blocks of eight keys.
-__device__ __forceinline__ void s8_unit(const unsigned char* stage, unsigned valid, const unsigned short (&meta)[4], const unsigned (&qf)[8][2],
-                                        const float (&f)[2], int lane, int box_shift, Sums8& s) {
+// One unit, whose boxes hold BOX tokens: `valid` has a bit for every key that counts (not 0), `scales` what its four blocks of eight keys are
+// to be multiplied by: the keys' scale, and the exponent of the values'. Keys and values lie as [box][keys, values][token][128], in
+// TMA's swizzle (16-byte piece c of token i at c ^ (i & 7)).
+template <int BOX>
+__device__ __forceinline__ void s8_unit(const unsigned char* stage, unsigned valid, const float2 (&scales)[4], const unsigned (&qf)[8][2],
+                                        const float (&f)[2], int lane, Sums8& s) {
     const int g = lane >> 2, t4 = lane & 3;
-    const int box_mask = (1 << box_shift) - 1;
-    // 16 bytes of key row (kv 0) or value row (kv 1) `key`, piece `c`
-    auto piece = [&](int kv, int key, int c) {
-        const int i = key & box_mask;
-        return *reinterpret_cast<const uint4*>(stage + (((key >> box_shift) * 2 + kv) << (box_shift + 7)) + i * S8_D + ((c ^ (i & 7)) << 4));
-    };
     const int row_key = (g >> 1) + ((g & 1) << 2);
+    auto token = [](int kv, int key) { return ((key / BOX) * 2 + kv) * BOX * S8_D + (key % BOX) * S8_D; };     // of multiples of 8: known here
+    const unsigned char* k_at[2] = {stage + row_key * S8_D + ((t4 ^ row_key) << 4), stage + row_key * S8_D + (((4 + t4) ^ row_key) << 4)};
+    const int v_key = t4 + ((g & 1) << 2);                       // the lane's own order of keys t4 and t4 + 4
+    const unsigned char* v_at[2] = {stage + v_key * S8_D + ((g ^ v_key) << 4), stage + (v_key ^ 4) * S8_D + ((g ^ v_key ^ 4) << 4)};
+    auto piece = [](const unsigned char* at) { return *reinterpret_cast<const uint4*>(at); };
     float t[2][4];
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
         float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};        // two chains of products
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const uint4 lo = piece(0, tile * 16 + row_key, half * 4 + t4), hi = piece(0, tile * 16 + 8 + row_key, half * 4 + t4);
+            const uint4 lo = piece(k_at[half] + token(0, tile * 16)), hi = piece(k_at[half] + token(0, tile * 16 + 8));
             const unsigned a[4] = {lo.x, lo.y, lo.z, lo.w}, b[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w)
                 s8_mma(w & 1 ? odd : even, kv8_half2((unsigned short)a[w]), kv8_half2((unsigned short)b[w]), kv8_half2((unsigned short)(a[w] >> 16)),
                        kv8_half2((unsigned short)(b[w] >> 16)), qf[half * 4 + w][0], qf[half * 4 + w][1]);
         }
-        const float k0 = kv8_scale(meta[tile * 2] & 0xffu), k1 = kv8_scale(meta[tile * 2 + 1] & 0xffu);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) t[tile][c] = (even[c] + odd[c]) * (c < 2 ? k0 : k1) * f[c & 1];
+        for (int c = 0; c < 4; ++c) t[tile][c] = (even[c] + odd[c]) * scales[tile * 2 + (c >> 1)].x * f[c & 1];
     }
     if (valid != 0xffffffffu) {
 #pragma unroll
@@ -191,7 +199,7 @@ __device__ __forceinline__ void s8_unit(const unsigned char* stage, unsigned val
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) u[tile][c] = t[tile][c] + (float)((int)(meta[tile * 2 + (c >> 1)] >> 8) - 127);
+        for (int c = 0; c < 4; ++c) u[tile][c] = t[tile][c] + scales[tile * 2 + (c >> 1)].y;
     float top[2], utop[2];
     bool raise = false;
 #pragma unroll
@@ -228,11 +236,11 @@ __device__ __forceinline__ void s8_unit(const unsigned char* stage, unsigned val
         s.l[1] += s8_ex2(t[tile][1] - m1) + s8_ex2(t[tile][3] - m1);
         const unsigned b0 = s8_transpose(s8_half2(s8_ex2(u[tile][0] - mu0), s8_ex2(u[tile][1] - mu1)));
         const unsigned b1 = s8_transpose(s8_half2(s8_ex2(u[tile][2] - mu0), s8_ex2(u[tile][3] - mu1)));
-        // keys t4 and t4 + 4 of both blocks of eight, the lane's own order first
-        const int key = tile * 16 + t4 + ((g & 1) << 2);
-        uint4 p0 = piece(1, key, g), p1 = piece(1, key ^ 4, g), p2 = piece(1, key + 8, g), p3 = piece(1, (key ^ 4) + 8, g);
+        uint4 p0 = piece(v_at[0] + token(1, tile * 16)), p1 = piece(v_at[1] + token(1, tile * 16));
+        uint4 p2 = piece(v_at[0] + token(1, tile * 16 + 8)), p3 = piece(v_at[1] + token(1, tile * 16 + 8));
         if (valid != 0xffffffffu) {                              // what lies in hidden places may be no number: 0 * NaN
             const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+            const int key = tile * 16 + v_key;
             if (!((valid >> key) & 1u)) p0 = none;
             if (!((valid >> (key ^ 4)) & 1u)) p1 = none;
             if (!((valid >> (key + 8)) & 1u)) p2 = none;
@@ -258,46 +266,58 @@ __device__ __forceinline__ float s8_weight(float m, float common) { return m == 
 // The row's result from its sums. No keys: zeros.
 __device__ __forceinline__ float s8_result(float o, float l, float m, float mu) { return l == 0.f ? 0.f : o / l * exp2f(mu - m); }
 
-#define S8_SYNC() asm volatile("bar.sync 1, %0;\n" ::"n"(S8_WARPS * 32) : "memory")
+// Four columns of a row's result from its sums (8-byte aligned).
+__device__ __forceinline__ void s8_store(bf16* out, float4 o, float l, float m, float mu) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(s8_result(o.x, l, m, mu), s8_result(o.y, l, m, mu));
+    const __nv_bfloat162 b = __floats2bfloat162_rn(s8_result(o.z, l, m, mu), s8_result(o.w, l, m, mu));
+    *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
 
+// A group of `heads` rows from row (r, head) on that the blocks first_block .. first_block + by - 1 share (by 0: none).
+struct Shared8 {
+    int first_block, by, heads, r, head;
+};
+
+#define S8_SYNC() asm volatile("bar.sync 1, %0;\n" ::"n"(S8_WARPS * 32) : "memory")       // of the warps that compute
+
+template <int BOX>
 __global__ void __launch_bounds__(S8_THREADS, 1)
 decode_kv8_stream_kernel(const __grid_constant__ CUtensorMap map, const Stream8Params p) {
     extern __shared__ unsigned char s8_raw[];
-    __shared__ __align__(8) uint64_t full_bar[S8_STAGES], empty_bar[S8_STAGES];
-    __shared__ __align__(8) unsigned short metas[S8_STAGES][4];
+    __shared__ __align__(8) uint64_t full_bar[S8_WARPS * S8_DEPTH], empty_bar[S8_WARPS * S8_DEPTH];      // stage d * S8_WARPS + w: warp w's
+    __shared__ __align__(16) float2 unit_scales[S8_WARPS * S8_DEPTH][4];
     __shared__ float wm[S8_WARPS][S8_HEADS], wmu[S8_WARPS][S8_HEADS], wl[S8_WARPS][S8_HEADS];
     __shared__ int pre[S8_MAX_ROWS + 1], ctxs[S8_MAX_ROWS];      // places of the requests before r, for one group; contexts
-    __shared__ unsigned arrived_before;
+    __shared__ int longest;
+    __shared__ Shared8 shared[2];                                // this block's part of a group that began earlier, of one that goes on later
     const uint32_t raw_addr = tc_smem_u32(s8_raw);
     unsigned char* ring = s8_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-    float* Ow = reinterpret_cast<float*>(ring + (size_t)S8_STAGES * S8_STAGE_BYTES);   // [warps][8][S8_OSTRIDE]
+    float* Ow = reinterpret_cast<float*>(ring + (size_t)S8_WARPS * S8_DEPTH * S8_STAGE_BYTES);      // [warps][8][S8_OSTRIDE]
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = p.nq / p.nkv, chunks = (G + S8_HEADS - 1) / S8_HEADS, groups = p.nkv * chunks;
 
-    if (tid == 0) {
-#pragma unroll
-        for (int s = 0; s < S8_STAGES; ++s) {
-            mbar_init(&full_bar[s], 2);                          // the boxes, and the scale bytes
-            mbar_init(&empty_bar[s], 1);
-        }
+    if (tid < S8_WARPS * S8_DEPTH) {
+        mbar_init(&full_bar[tid], 2);                            // the boxes, and the scales
+        mbar_init(&empty_bar[tid], 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
-        pre[0] = 0;
     }
+    if (tid == 32) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
+    if (tid == 0) pre[0] = 0;
+    if (tid < 2) shared[tid].by = 0;
     pdl_trigger();
     pdl_wait();
-    for (int r = tid; r < p.R; r += S8_THREADS) {
-        int ctx = p.ctx_len[r];
-        ctx = ctx < 0 ? 0 : (ctx < p.max_ctx ? ctx : p.max_ctx);
-        ctxs[r] = ctx;
-        pre[r + 1] = s8_units(ctx, p.window) + S8_GROUP_COST;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        int carry = 0;
+    if (warp == 0) {                                             // places, their running sums, the longest group
+        int carry = 0, most = 0;
         for (int base = 0; base < p.R; base += 32) {
-            int val = base + lane < p.R ? pre[base + lane + 1] : 0;
+            int val = 0;
+            if (base + lane < p.R) {
+                int ctx = p.ctx_len[base + lane];
+                ctx = ctx < 0 ? 0 : (ctx < p.max_ctx ? ctx : p.max_ctx);
+                ctxs[base + lane] = ctx;
+                val = s8_units(ctx, p.window) + S8_GROUP_COST;
+            }
+            most = max(most, val);
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, val, off);
@@ -306,89 +326,130 @@ decode_kv8_stream_kernel(const __grid_constant__ CUtensorMap map, const Stream8P
             if (base + lane < p.R) pre[base + lane + 1] = val + carry;
             carry += __shfl_sync(0xffffffffu, val, 31);
         }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) longest = most - S8_GROUP_COST;
     }
     __syncthreads();
 
+    // How the list is dealt out: evenly, or (few groups of about the same length) every group to `split` blocks of its own, which
+    // spares most blocks a second group and the borders that fall inside groups.
     const long N = (long)groups * pre[p.R];
     const long most = N / S8_MIN_SHARE > 0 ? N / S8_MIN_SHARE : 1;
     const long blocks = (long)gridDim.x < most ? (long)gridDim.x : most;
-    if ((long)blockIdx.x >= blocks) return;
-    const long x0 = (long)blockIdx.x * N / blocks, x1 = ((long)blockIdx.x + 1) * N / blocks;
-    Seg8 seg = s8_open(x0, x1, pre, ctxs, p.R, groups, p.window);
+    const int all = p.R * groups;
+    int split = 0;
+    if (all <= (int)gridDim.x) {
+        split = min((int)gridDim.x / all, (longest + S8_OWN_UNITS - 1) / S8_OWN_UNITS);
+        if ((longest + split - 1) / split > N / blocks + S8_EVEN_COST) split = 0;
+    }
+    Seg8 seg;
+    long x1 = 0;
+    if (split > 0) {
+        const int group = blockIdx.x / split, part = blockIdx.x % split;
+        if (group >= all) return;
+        seg.r = group / groups;
+        seg.h = group % groups;
+        s8_request(seg, pre, ctxs, p.window);
+        const int own = min(split, (seg.n + S8_OWN_UNITS - 1) / S8_OWN_UNITS);   // a short group takes fewer
+        if (part >= own) return;
+        seg.i0 = (int)((long)seg.n * part / own);
+        seg.i1 = (int)((long)seg.n * (part + 1) / own);
+        seg.ok = true;
+        seg.x = seg.x_end = x1 = 0;
+        if (tid == 0 && own > 1) shared[part == 0 ? 1 : 0] = Shared8{group * split, own, 0, 0, 0};
+    } else {
+        if ((long)blockIdx.x >= blocks) return;
+        x1 = ((long)blockIdx.x + 1) * N / blocks;
+        seg = s8_open((long)blockIdx.x * N / blocks, x1, pre, ctxs, p.R, groups, p.window);
+    }
 
-    if (warp == S8_WARPS) {
-        // ---- loads: eight units at a time, lane 4 u + b the block b of eight keys of unit u ----
+    if (warp >= S8_WARPS) {
+        // ---- loads: warp l of S8_LOADERS serves the units n with n mod S8_LOADERS = l, a few at a time: lane 4 u + b sees to block b of
+        // eight keys of the u-th of them. Page numbers are asked for two turns ahead, scale bytes one, so that neither is waited for
+        // while boxes could be on their way. ----
         const int u = lane >> 2, b = lane & 3;
-        const bool boxes = (b * 8) % p.box_tokens == 0;          // this lane issues a box
+        const bool boxes = (b * 8) % BOX == 0;                   // this lane issues a box
         const size_t body = (size_t)2 * p.nkv * p.page_size * S8_D;
-        int j = 0;                                               // units of the segment that are on their way
-        int count = 0, key = 0, kvh = 0, page = -1;              // the coming batch: its units; this lane's block, its page
+        struct Ask {
+            int key, head, page;
+            bool ok;
+        };
+        unsigned n_ahead = (unsigned)(warp - S8_WARPS) + u * S8_LOADERS;         // this lane's coming unit, counted from the block's first
+        unsigned before = 0;                                     // units of the block before `seg`
         auto fetch = [&]() {
-            count = 0;
-            if (!seg.ok) return;
-            count = min(seg.i1 - seg.i0 - j, 8);
-            kvh = seg.h / chunks;
-            key = (seg.first + seg.i0 + j + u) * S8_KEYS + b * 8;
-            page = -1;
-            if (u < count && key < seg.ctx) {
-                page = p.block_tables[(size_t)seg.r * p.table_stride + key / p.page_size];
-                if (page >= p.num_pages) page = -1;
-            }
-            j += count;
-            if (j == seg.i1 - seg.i0) {
+            Ask t;
+            while (seg.ok && n_ahead - before >= (unsigned)(seg.i1 - seg.i0)) {
+                before += seg.i1 - seg.i0;
                 s8_next(seg, x1, pre, ctxs, groups, p.window);
-                j = 0;
+            }
+            t.ok = seg.ok && u < S8_ASK;
+            t.page = -1;
+            t.key = (seg.first + seg.i0 + (int)(n_ahead - before)) * S8_KEYS + b * 8;
+            t.head = seg.h / chunks;
+            if (t.ok && t.key < seg.ctx) t.page = p.block_tables[(size_t)seg.r * p.table_stride + (t.key >> p.page_shift)];
+            n_ahead += S8_LOADERS * S8_ASK;
+            return t;
+        };
+        unsigned ek = 0u, ev = 0u;
+        auto scales = [&](Ask& t) {
+            if (t.page >= p.num_pages) t.page = -1;
+            if (t.page >= 0) {
+                const unsigned char* at = p.pages + (size_t)t.page * p.page_bytes + body + t.head;
+                ek = at[0];
+                ev = at[p.nkv];
             }
         };
-        fetch();
-        unsigned n0 = 0;
-        while (count > 0) {
-            const int now = count, at = key, head = kvh, id = page;
-            unsigned meta = 0xffffu;                             // a page that is missing
-            if (id >= 0) {
-                const unsigned char* scales = p.pages + (size_t)id * p.page_bytes + body + head;
-                meta = scales[0] | (unsigned)scales[p.nkv] << 8;
-            }
-            fetch();
-            if (u < now) {
-                const unsigned n = n0 + u, slot = n % S8_STAGES;
-                if (n >= S8_STAGES) mbar_wait(&empty_bar[slot], ((n / S8_STAGES) - 1) & 1, p.error_flag);
+        unsigned n = n_ahead;
+        Ask now = fetch(), next = fetch();
+        scales(now);
+        while (__any_sync(0xffffffffu, now.ok)) {
+            const Ask after = fetch();
+            const unsigned slot = n % (S8_WARPS * S8_DEPTH), round = n / (S8_WARPS * S8_DEPTH);
+            if (now.ok) {
+                if (round > 0) mbar_wait(&empty_bar[slot], (round - 1) & 1, p.error_flag);
                 if (b == 0) mbar_expect_tx(&full_bar[slot], S8_STAGE_BYTES);
             }
             __syncwarp();
-            if (u < now) {
-                const unsigned slot = (n0 + u) % S8_STAGES;
-                if (boxes)                                       // out of range: the box arrives as zeros
-                    s8_load_box(ring + (size_t)slot * S8_STAGE_BYTES + b * 8 * 2 * S8_D, &map, at % p.page_size, head, id >= 0 ? id : p.num_pages,
-                                &full_bar[slot]);
-                metas[slot][b] = (unsigned short)meta;
-            }
+            if (now.ok && boxes)                                 // out of range: the box arrives as zeros
+                s8_load_box(ring + (size_t)slot * S8_STAGE_BYTES + b * 8 * 2 * S8_D, &map, now.key & (p.page_size - 1), now.head,
+                            now.page >= 0 ? now.page : p.num_pages, &full_bar[slot]);
+            if (now.ok) unit_scales[slot][b] = make_float2(now.page >= 0 ? kv8_scale(ek) : -1.f, (float)((int)ev - 127));      // -1: a page that is missing
             __syncwarp();
-            if (u < now && b == 0)
-                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(tc_smem_u32(&full_bar[(n0 + u) % S8_STAGES])) : "memory");
-            n0 += now;
+            if (now.ok && b == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(tc_smem_u32(&full_bar[slot])) : "memory");
+            n += S8_LOADERS * S8_ASK;
+            now = next;
+            next = after;
+            scales(now);
         }
         return;
     }
 
-    // ---- compute ----
+    // ---- compute: unit n of the block is warp n mod S8_WARPS's ----
     const int g = lane >> 2, t4 = lane & 3;
-    const int box_shift = 31 - __clz(p.box_tokens);
-    unsigned n0 = 0;
+    int at = warp;                                               // the coming unit of `seg`, counted from its i0
+    unsigned k = 0;                                              // this warp's units so far
+    uint4 q_raw[4];                                              // entries 16 t4 .. 16 t4 + 15 of either half of query head g
+    auto ask_q = [&](const Seg8& of) {
+        const int head = (of.h % chunks) * S8_HEADS + g;         // within the group that shares a key/value head
+        const bf16* q = p.q + (size_t)of.r * p.q_stride + (size_t)(of.h / chunks * G + head) * S8_D + t4 * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q_raw[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (of.ok && head < G) q_raw[i] = *reinterpret_cast<const uint4*>(q + (i >> 1) * 64 + (i & 1) * 8);
+        }
+    };
+    ask_q(seg);
     while (seg.ok) {
         const int r = seg.r, kvh = seg.h / chunks, head0 = (seg.h % chunks) * S8_HEADS;
         const int heads = min(G - head0, S8_HEADS);
-        // this lane's part of query head g: entries 16 t4 .. 16 t4 + 15 of either half
+        // this lane's part of query head g, which was asked for before the segment before this one ended
         unsigned qf[8][2];
         float f[2];
         {
             float x[32], amax = 0.f;
-            const bf16* q = p.q + (size_t)r * p.q_stride + (size_t)(kvh * G + head0 + g) * S8_D + t4 * 16;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-                if (g < heads) raw = *reinterpret_cast<const uint4*>(q + (i >> 1) * 64 + (i & 1) * 8);
-                const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+                const unsigned w[4] = {q_raw[i].x, q_raw[i].y, q_raw[i].z, q_raw[i].w};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     x[i * 8 + 2 * c] = __uint_as_float(w[c] << 16);
@@ -418,129 +479,138 @@ decode_kv8_stream_kernel(const __grid_constant__ CUtensorMap map, const Stream8P
         s.l[0] = s.l[1] = 0.f;
         const int units = seg.i1 - seg.i0;
         const int low = p.window > 0 ? seg.ctx - p.window : 0;   // the first key that counts
-        for (int i = (int)((warp - n0) & (S8_WARPS - 1)); i < units; i += S8_WARPS) {
-            const unsigned n = n0 + i, slot = n % S8_STAGES;
-            mbar_wait(&full_bar[slot], (n / S8_STAGES) & 1, p.error_flag);
-            const int key0 = (seg.first + seg.i0 + i) * S8_KEYS;
-            const uint2 raw = *reinterpret_cast<const uint2*>(metas[slot]);
-            const unsigned short meta[4] = {(unsigned short)raw.x, (unsigned short)(raw.x >> 16), (unsigned short)raw.y, (unsigned short)(raw.y >> 16)};
+        for (; at < units; at += S8_WARPS, ++k) {
+            const unsigned slot = k % S8_DEPTH * S8_WARPS + warp;
+            mbar_wait(&full_bar[slot], (k / S8_DEPTH) & 1, p.error_flag);
+            const float4 s01 = reinterpret_cast<const float4*>(unit_scales[slot])[0], s23 = reinterpret_cast<const float4*>(unit_scales[slot])[1];
+            const float2 scales[4] = {make_float2(s01.x, s01.y), make_float2(s01.z, s01.w), make_float2(s23.x, s23.y), make_float2(s23.z, s23.w)};
+            const int key0 = (seg.first + seg.i0 + at) * S8_KEYS;
             unsigned valid = 0xffffffffu;
             if (seg.ctx - key0 < S8_KEYS) valid = seg.ctx > key0 ? (1u << (seg.ctx - key0)) - 1u : 0u;
             if (low > key0) valid = low - key0 < S8_KEYS ? valid & ~((1u << (low - key0)) - 1u) : 0u;
 #pragma unroll
             for (int b = 0; b < 4; ++b)
-                if (meta[b] == 0xffffu) valid &= ~(0xffu << (8 * b));
-            if (valid != 0u) s8_unit(ring + (size_t)slot * S8_STAGE_BYTES, valid, meta, qf, f, lane, box_shift, s);
-            __syncwarp();
+                if (scales[b].x < 0.f) valid &= ~(0xffu << (8 * b));
+            if (valid != 0u) s8_unit<BOX>(ring + (size_t)slot * S8_STAGE_BYTES, valid, scales, qf, f, lane, s);
+            __syncwarp();                                        // the stage is read: it may be filled again
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(tc_smem_u32(&empty_bar[slot])) : "memory");
         }
-        n0 += units;
+        at -= units;
 
-        // ---- the segment is read: the warps' sums ----
+        // ---- the segment is read: the warps' maxima, then their sums under the largest ----
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], o);
-            float* row = Ow + ((size_t)warp * S8_HEADS + 2 * t4 + h) * S8_OSTRIDE + g * 16;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float4*>(row + 4 * i) = make_float4(s.o[2 * i][h], s.o[2 * i][2 + h], s.o[2 * i + 1][h], s.o[2 * i + 1][2 + h]);
+        for (int h = 0; h < 2; ++h)
             if (g == 0) {
                 wm[warp][2 * t4 + h] = s.m[h];
                 wmu[warp][2 * t4 + h] = s.mu[h];
-                wl[warp][2 * t4 + h] = s.l[h];
             }
-        }
         S8_SYNC();
-        const bool whole = seg.i0 == 0 && seg.i1 == seg.n;
-        int first_block = 0, shared_by = 1;
-        float* part = nullptr;
-        if (!whole) {
-            const long xg = seg.x - seg.i0;                      // the group's first place in the list
-            first_block = (int)(((xg + 1) * blocks - 1) / N);    // the last block whose share starts at or before a place
-            shared_by = (int)(((xg + seg.n) * blocks - 1) / N) - first_block + 1;
-            part = p.partials + ((size_t)blockIdx.x * 2 + (seg.i0 > 0 ? 0 : 1)) * S8_PART;
-        }
-        const int col = tid & (S8_D - 1);
-        bf16* out = p.out + (size_t)r * p.out_stride + (size_t)(kvh * G + head0) * S8_D + col;
-        for (int row = tid >> 7; row < heads; row += S8_WARPS * 32 / S8_D) {
-            float m = wm[0][row], mu = wmu[0][row];
+        float top[2], utop[2];
 #pragma unroll
-            for (int w = 1; w < S8_WARPS; ++w) {
-                m = fmaxf(m, wm[w][row]);
-                mu = fmaxf(mu, wmu[w][row]);
-            }
-            float acc = 0.f, l = 0.f;
+        for (int h = 0; h < 2; ++h) {
+            top[h] = utop[h] = -INFINITY;
 #pragma unroll
             for (int w = 0; w < S8_WARPS; ++w) {
-                acc = fmaf(Ow[((size_t)w * S8_HEADS + row) * S8_OSTRIDE + col], s8_weight(wmu[w][row], mu), acc);
-                l = fmaf(wl[w][row], s8_weight(wm[w][row], m), l);
+                top[h] = fmaxf(top[h], wm[w][2 * t4 + h]);
+                utop[h] = fmaxf(utop[h], wmu[w][2 * t4 + h]);
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], o);
+            const float weight = s8_weight(s.mu[h], utop[h]);
+            float* row = Ow + ((size_t)warp * S8_HEADS + 2 * t4 + h) * S8_OSTRIDE + g * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(row + 4 * i) = make_float4(s.o[2 * i][h] * weight, s.o[2 * i][2 + h] * weight, s.o[2 * i + 1][h] * weight,
+                                                                      s.o[2 * i + 1][2 + h] * weight);
+            if (g == 0) wl[warp][2 * t4 + h] = s.l[h] * s8_weight(s.m[h], top[h]);
+        }
+        S8_SYNC();
+        Seg8 after = seg;
+        s8_next(after, x1, pre, ctxs, groups, p.window);
+        ask_q(after);
+        const bool whole = seg.i0 == 0 && seg.i1 == seg.n;
+        if (!whole && tid == 0) {
+            Shared8& of = shared[seg.i0 > 0 ? 0 : 1];
+            if (split == 0) {
+                const long xg = seg.x - seg.i0;                  // the group's first place in the list
+                of.first_block = (int)(((xg + 1) * blocks - 1) / N);     // the last block whose share starts at or before a place
+                of.by = (int)(((xg + seg.n) * blocks - 1) / N) - of.first_block + 1;
+            }
+            of.heads = heads;
+            of.r = r;
+            of.head = kvh * G + head0;
+        }
+        if (warp < heads) {                                      // a warp takes a row, a lane four columns
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f, m = -INFINITY, mu = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < S8_WARPS; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(Ow + ((size_t)w * S8_HEADS + warp) * S8_OSTRIDE + lane * 4);
+                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+                l += wl[w][warp];
+                m = fmaxf(m, wm[w][warp]);
+                mu = fmaxf(mu, wmu[w][warp]);
             }
             if (whole) {
-                out[row * S8_D] = __float2bfloat16_rn(s8_result(acc, l, m, mu));
+                s8_store(p.out + (size_t)r * p.out_stride + (size_t)(kvh * G + head0 + warp) * S8_D + lane * 4, o, l, m, mu);
             } else {
-                part[row * S8_D + col] = acc;
-                if (col == 0) {
-                    part[S8_HEADS * S8_D + row] = m;
-                    part[S8_HEADS * S8_D + S8_HEADS + row] = mu;
-                    part[S8_HEADS * S8_D + 2 * S8_HEADS + row] = l;
-                }
-            }
-        }
-        if (!whole) {
-            __threadfence();                                     // the sums are visible before the count is
-            S8_SYNC();
-            if (tid == 0) arrived_before = atomicAdd(&p.arrivals[first_block], 1u);
-            S8_SYNC();
-            if (arrived_before == (unsigned)(shared_by - 1)) {
-                __threadfence();
-                // the first block's segment goes on later, the others' began earlier
-                auto part_of = [&](int k) { return p.partials + ((size_t)(first_block + k) * 2 + (k == 0 ? 1 : 0)) * S8_PART; };
-                float* ml = Ow;                                  // [shared_by][m of 8 rows | mu | l]: at most 256 * 24 floats
-                for (int e = tid; e < shared_by * 3 * S8_HEADS; e += S8_WARPS * 32) {
-                    const int k = e / (3 * S8_HEADS);
-                    ml[e] = __ldcg(part_of(k) + S8_HEADS * S8_D + (e - k * 3 * S8_HEADS));
-                }
-                S8_SYNC();
-                constexpr int ROWS = S8_HEADS * S8_D / (S8_WARPS * 32);          // rows of a thread: 4
-                const int row0 = tid >> 7;
-                float m[ROWS], mu[ROWS], l[ROWS], acc[ROWS];
-#pragma unroll
-                for (int i = 0; i < ROWS; ++i) {
-                    m[i] = mu[i] = -INFINITY;
-                    l[i] = acc[i] = 0.f;
-                }
-                for (int k = 0; k < shared_by; ++k)
-#pragma unroll
-                    for (int i = 0; i < ROWS; ++i) {
-                        m[i] = fmaxf(m[i], ml[k * 3 * S8_HEADS + row0 + 2 * i]);
-                        mu[i] = fmaxf(mu[i], ml[k * 3 * S8_HEADS + S8_HEADS + row0 + 2 * i]);
-                    }
-                for (int k0 = 0; k0 < shared_by; k0 += 4) {
-                    float val[4][ROWS];
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-#pragma unroll
-                        for (int i = 0; i < ROWS; ++i)
-                            val[v][i] = k0 + v < shared_by && row0 + 2 * i < heads ? __ldcg(part_of(k0 + v) + (row0 + 2 * i) * S8_D + col) : 0.f;
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        if (k0 + v < shared_by)
-#pragma unroll
-                            for (int i = 0; i < ROWS; ++i) {
-                                const float* of = ml + (k0 + v) * 3 * S8_HEADS + row0 + 2 * i;
-                                acc[i] = fmaf(val[v][i], s8_weight(of[S8_HEADS], mu[i]), acc[i]);
-                                l[i] = fmaf(of[2 * S8_HEADS], s8_weight(of[0], m[i]), l[i]);
-                            }
-                }
-#pragma unroll
-                for (int i = 0; i < ROWS; ++i)
-                    if (row0 + 2 * i < heads) out[(row0 + 2 * i) * S8_D] = __float2bfloat16_rn(s8_result(acc[i], l[i], m[i], mu[i]));
-                if (tid == 0) p.arrivals[first_block] = 0u;      // for the next launch
+                float* part = p.partials + ((size_t)blockIdx.x * 2 + (seg.i0 > 0 ? 0 : 1)) * S8_PART;
+                *reinterpret_cast<float4*>(part + warp * S8_D + lane * 4) = o;
+                if (lane == 0) *reinterpret_cast<float4*>(part + S8_HEADS * S8_D + warp * 4) = make_float4(m, mu, l, 0.f);
             }
         }
         S8_SYNC();                                               // the sums are read: the next segment may write its own
-        s8_next(seg, x1, pre, ctxs, groups, p.window);
+        seg = after;
+    }
+
+    // ---- groups that this block shares with others: counted once all its own are read (one thread's fence covers what the block
+    // wrote before the barrier), and those added up that it is the last to count on ----
+    S8_SYNC();
+    if (tid < 2 && shared[tid].by > 0) {
+        __threadfence();
+        const unsigned before = atomicAdd(&p.arrivals[shared[tid].first_block], 1u);
+        __threadfence();
+        if (before != (unsigned)(shared[tid].by - 1)) shared[tid].by = 0;
+    }
+    S8_SYNC();
+    for (int which = 0; which < 2; ++which) {
+        const Shared8 of = shared[which];
+        if (of.by == 0 || warp >= of.heads) continue;
+        // the first block's segment goes on later, the others' began earlier
+        auto part_of = [&](int b) { return p.partials + ((size_t)(of.first_block + b) * 2 + (b == 0 ? 1 : 0)) * S8_PART; };
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f, m = -INFINITY, mu = -INFINITY;
+        for (int b0 = 0; b0 < of.by; b0 += 4) {                  // four blocks at a time, what they left on its way together
+            float4 v[4], ml[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                ml[b] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+                v[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (b0 + b < of.by) {
+                    v[b] = __ldcg(reinterpret_cast<const float4*>(part_of(b0 + b) + warp * S8_D) + lane);
+                    ml[b] = __ldcg(reinterpret_cast<const float4*>(part_of(b0 + b) + S8_HEADS * S8_D) + warp);
+                }
+            }
+            float m_new = m, mu_new = mu;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                m_new = fmaxf(m_new, ml[b].x);
+                mu_new = fmaxf(mu_new, ml[b].y);
+            }
+            l *= s8_weight(m, m_new);
+            const float old = s8_weight(mu, mu_new);
+            o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                l = fmaf(ml[b].z, s8_weight(ml[b].x, m_new), l);
+                const float w = s8_weight(ml[b].y, mu_new);
+                o.x = fmaf(v[b].x, w, o.x); o.y = fmaf(v[b].y, w, o.y); o.z = fmaf(v[b].z, w, o.z); o.w = fmaf(v[b].w, w, o.w);
+            }
+            m = m_new;
+            mu = mu_new;
+        }
+        s8_store(p.out + (size_t)of.r * p.out_stride + (size_t)(of.head + warp) * S8_D + lane * 4, o, l, m, mu);
+        if (tid == 0) p.arrivals[of.first_block] = 0u;           // for the next launch
     }
 }
 
@@ -548,7 +618,7 @@ decode_kv8_stream_kernel(const __grid_constant__ CUtensorMap map, const Stream8P
 // Sizes the kernel takes (bfloat16 queries whose rows start on 16 bytes), the scratch it needs and its counters, which are zero before
 // a launch and after it; launches that may run at the same time need scratch and counters of their own.
 LLMP_API int llmp_kv8_stream_supports(int nq, int nkv, int d, int page_size) {
-    return d == S8_D && nkv > 0 && nq % nkv == 0 && (page_size == 8 || page_size == 16 || (page_size > 0 && page_size % 32 == 0));
+    return d == S8_D && nkv > 0 && nq % nkv == 0 && page_size >= 8 && (page_size & (page_size - 1)) == 0;
 }
 LLMP_API long llmp_kv8_stream_scratch_floats() { return (long)S8_MAX_BLOCKS * 2 * S8_PART; }
 LLMP_API int llmp_kv8_stream_counters() { return S8_MAX_BLOCKS; }
@@ -559,43 +629,48 @@ LLMP_API int llmp_kv8_stream(const void* q, long q_stride, void* out, long out_s
     if (R <= 0) return 0;
     LLMP_REQUIRE(llmp_kv8_stream_supports(nq, nkv, S8_D, page_size), "kv8 attention: %d and %d heads, pages of %d tokens are not for this kernel", nq, nkv, page_size);
     LLMP_REQUIRE(num_pages > 0 && max_ctx > 0 && table_stride > 0, "kv8 attention: bad context %d or tables", max_ctx);
-    LLMP_REQUIRE((q_stride % 8) == 0 && ((size_t)q % 16) == 0 && ((size_t)pages % 16) == 0, "kv8 attention: rows must be 16-byte aligned");
+    LLMP_REQUIRE((q_stride % 8) == 0 && ((size_t)q % 16) == 0 && ((size_t)pages % 16) == 0 && ((size_t)out % 8) == 0 && (out_stride % 4) == 0, "kv8 attention: rows must be 16-byte aligned");
     LLMP_REQUIRE(scratch != nullptr && scratch_floats >= llmp_kv8_stream_scratch_floats() && counters != nullptr && error_flag != nullptr,
                  "kv8 attention: scratch, counters and an error flag are needed");
-    static int sms = 0;
-    if (sms == 0) {
+    static int blocks = 0;
+    if (blocks == 0) {
         int dev = 0, n = 0;
         cudaGetDevice(&dev);
         cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-        sms = n <= 0 ? 148 : (n > S8_MAX_BLOCKS ? S8_MAX_BLOCKS : n);
+        n = n <= 0 ? 148 : n;
+        blocks = n > S8_MAX_BLOCKS ? S8_MAX_BLOCKS : n;
     }
     Stream8Params p;
     p.pages = (const unsigned char*)pages;
     p.q_stride = q_stride; p.out_stride = out_stride; p.page_bytes = kv8_page_bytes(nkv, page_size, S8_D); p.table_stride = table_stride;
     const long held = (long)table_stride * page_size;            // what a row of the tables has room for
     p.num_pages = num_pages; p.max_ctx = held < max_ctx ? (int)held : max_ctx; p.nq = nq; p.nkv = nkv; p.page_size = page_size;
-    p.box_tokens = page_size < S8_KEYS ? page_size : S8_KEYS; p.window = window; p.scale = scale; p.partials = scratch; p.arrivals = counters;
+    p.page_shift = 31 - __builtin_clz((unsigned)page_size); p.window = window; p.scale = scale; p.partials = scratch; p.arrivals = counters;
     p.error_flag = error_flag;
+    const int box_tokens = page_size < S8_KEYS ? page_size : S8_KEYS;
     EncodeTiledFn encode = llmp_tensor_map_encoder();
     LLMP_REQUIRE(encode != nullptr, "kv8 attention: the driver does not provide cuTensorMapEncodeTiled");
     CUtensorMap map;
     const cuuint64_t row = S8_D, plane = row * page_size;
     const cuuint64_t dims[5] = {S8_D, (cuuint64_t)page_size, (cuuint64_t)nkv, 2, (cuuint64_t)num_pages};
     const cuuint64_t strides[4] = {row, plane, plane * nkv, (cuuint64_t)p.page_bytes};
-    const cuuint32_t box[5] = {S8_D, (cuuint32_t)p.box_tokens, 1, 2, 1};
+    const cuuint32_t box[5] = {S8_D, (cuuint32_t)box_tokens, 1, 2, 1};
     const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
     const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     LLMP_REQUIRE(rc == CUDA_SUCCESS, "kv8 attention: cuTensorMapEncodeTiled failed with code %d", (int)rc);
-    const size_t smem = (size_t)S8_STAGES * S8_STAGE_BYTES + sizeof(float) * S8_WARPS * S8_HEADS * S8_OSTRIDE + 1024;
-    LLMP_ALLOW_SMEM(decode_kv8_stream_kernel, smem);
+    const size_t smem = (size_t)S8_WARPS * S8_DEPTH * S8_STAGE_BYTES + sizeof(float) * S8_WARPS * S8_HEADS * S8_OSTRIDE + 1024;
+    const auto kernel = box_tokens == 8 ? decode_kv8_stream_kernel<8> : box_tokens == 16 ? decode_kv8_stream_kernel<16> : decode_kv8_stream_kernel<32>;
+    if (box_tokens == 8) LLMP_ALLOW_SMEM(decode_kv8_stream_kernel<8>, smem);
+    else if (box_tokens == 16) LLMP_ALLOW_SMEM(decode_kv8_stream_kernel<16>, smem);
+    else LLMP_ALLOW_SMEM(decode_kv8_stream_kernel<32>, smem);
     for (int r = 0; r < R; r += S8_MAX_ROWS) {                   // launches that follow one another may share scratch and counters
         p.q = (const bf16*)q + (size_t)r * q_stride;
         p.out = (bf16*)out + (size_t)r * out_stride;
         p.block_tables = block_tables + (size_t)r * table_stride;
         p.ctx_len = ctx_len + r;
         p.R = R - r < S8_MAX_ROWS ? R - r : S8_MAX_ROWS;
-        llmp_launch_dependent(decode_kv8_stream_kernel, dim3((unsigned)sms), dim3(S8_THREADS), smem, stream, map, p);
+        llmp_launch_dependent(kernel, dim3((unsigned)blocks), dim3(S8_THREADS), smem, stream, map, p);
     }
     return llmp_check_launch("kv8_stream");
 }

@@ -10,9 +10,11 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from typing import Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from ..cache.spec import kv8_page_bytes
@@ -2303,19 +2305,27 @@ def wkv_gate(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, out: tor
 
 
 # ---- keys and values in 8 bits, and copies of pages ------------------------------------------------------------------------
+# (Steps of single tokens make these calls for every layer: messages are made only where they are raised.)
 def _on_current_device(*tensors: torch.Tensor) -> None:
+    """Kernels run on the current device: an error for a tensor that is anywhere else."""
+    here = None
     for t in tensors:
-        if t.is_cuda and t.device.index != _device():
-            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{_device()}")
+        at = t.get_device()
+        if at < 0:
+            raise KernelError("a kernel was given a tensor that is not on a CUDA device; this engine has no CPU path")
+        if here is None:
+            here = _device()
+        if at != here:
+            raise KernelError(f"a tensor is on cuda:{at}, the current device is cuda:{here}")
 
 
 def _kv8_pages(pages: torch.Tensor, num_kv_heads: int, head_dim: int, page_size: int) -> None:
-    _need(num_kv_heads > 0 and page_size > 0 and 16 <= head_dim <= 256 and head_dim % 16 == 0,
-          "8-bit pages take head sizes that are multiples of 16 in 16..256, and at least one head and token")
-    _need(pages.dtype == torch.uint8 and pages.dim() == 2 and pages.is_contiguous() and pages.shape[0] > 0 and
-          pages.shape[1] == kv8_page_bytes(num_kv_heads, page_size, head_dim),
-          f"8-bit pages must be contiguous uint8 [pages, {kv8_page_bytes(num_kv_heads, page_size, head_dim)}] for {num_kv_heads} heads of "
-          f"{head_dim} and {page_size} tokens")
+    if not (num_kv_heads > 0 and page_size > 0 and 16 <= head_dim <= 256 and head_dim % 16 == 0):
+        raise KernelError("8-bit pages take head sizes that are multiples of 16 in 16..256, and at least one head and token")
+    if not (pages.dtype == torch.uint8 and pages.dim() == 2 and pages.is_contiguous() and pages.shape[0] > 0 and
+            pages.shape[1] == kv8_page_bytes(num_kv_heads, page_size, head_dim)):
+        raise KernelError(f"8-bit pages must be contiguous uint8 [pages, {kv8_page_bytes(num_kv_heads, page_size, head_dim)}] for {num_kv_heads} "
+                          f"heads of {head_dim} and {page_size} tokens")
 
 
 def kv8_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor, num_kv_heads: int, head_dim: int,
@@ -2328,12 +2338,13 @@ def kv8_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torc
     _kv8_pages(pages, num_kv_heads, head_dim, page_size)
     _i32(slots, "slots")
     N = slots.numel()
-    _need(k.dim() == 2 and k.shape == (N, num_kv_heads * head_dim) and v.shape == k.shape and k.dtype == v.dtype,
-          "keys and values must be [tokens, kv heads * head_dim] of one type, one row per slot")
-    _need(N <= 1 or (k.stride(1) == 1 and v.stride(1) == 1), "the entries of a row of keys or values must be neighbours")
-    _on_current_device(k, v, slots, pages)
+    if not (k.dim() == 2 and k.shape == (N, num_kv_heads * head_dim) and v.shape == k.shape and k.dtype == v.dtype):
+        raise KernelError("keys and values must be [tokens, kv heads * head_dim] of one type, one row per slot")
+    if N > 1 and not (k.stride(1) == 1 and v.stride(1) == 1):
+        raise KernelError("the entries of a row of keys or values must be neighbours")
     dtype = dtype_code(k.dtype)
-    _call("llmp_kv8_store", _ptr(k), k.stride(0), _ptr(v), v.stride(0), dtype, _ptr(slots), _ptr(pages), pages.shape[0], N,
+    _on_current_device(k, v, slots, pages)
+    _call("llmp_kv8_store", k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), dtype, slots.data_ptr(), pages.data_ptr(), pages.shape[0], N,
           num_kv_heads, head_dim, page_size, _stream())
 
 
@@ -2341,17 +2352,21 @@ def kv8_gather(pages: torch.Tensor, block_tables: torch.Tensor, ctx_len: torch.T
     """out[i] (``[n, 2, kv heads, page_size, head_dim]``, float32 or bfloat16, exact in either) = the values of the 8-bit page
     that entry ``index[i]`` of the flattened ``block_tables`` names; zeros behind the request's last token and for a page that
     is missing."""
-    _need(out.dim() == 5 and out.shape[1] == 2 and out.is_contiguous(), "unpacked pages must be contiguous [n, 2, kv heads, page_size, head_dim]")
-    nkv, page_size, d = out.shape[2:]
+    if not (out.dim() == 5 and out.shape[1] == 2 and out.is_contiguous()):
+        raise KernelError("unpacked pages must be contiguous [n, 2, kv heads, page_size, head_dim]")
+    n, _two, nkv, page_size, d = out.shape
     _kv8_pages(pages, nkv, d, page_size)
-    for name, t in (("block_tables", block_tables), ("ctx_len", ctx_len), ("index", index)):
-        _i32(t, name)
-    _need(block_tables.dim() == 2 and block_tables.shape[0] == ctx_len.numel(), "block tables must be [requests, pages]")
-    _need(index.numel() == out.shape[0], "one index per unpacked page")
-    _on_current_device(pages, block_tables, ctx_len, index, out)
+    _i32(block_tables, "block_tables")
+    _i32(ctx_len, "ctx_len")
+    _i32(index, "index")
+    if block_tables.dim() != 2 or block_tables.shape[0] != ctx_len.numel():
+        raise KernelError("block tables must be [requests, pages]")
+    if index.numel() != n:
+        raise KernelError("one index per unpacked page")
     dtype = dtype_code(out.dtype)
-    _call("llmp_kv8_gather", _ptr(pages), pages.shape[0], _ptr(block_tables), ctx_len.numel(), block_tables.shape[1], _ptr(ctx_len),
-          _ptr(index), index.numel(), _ptr(out), dtype, nkv, d, page_size, _stream())
+    _on_current_device(pages, block_tables, ctx_len, index, out)
+    _call("llmp_kv8_gather", pages.data_ptr(), pages.shape[0], block_tables.data_ptr(), ctx_len.numel(), block_tables.shape[1], ctx_len.data_ptr(),
+          index.data_ptr(), n, out.data_ptr(), dtype, nkv, d, page_size, _stream())
     return out
 
 
@@ -2368,29 +2383,40 @@ def kv8_stream_supports(dtype: torch.dtype, num_heads: int, num_kv_heads: int, h
     return dtype == torch.bfloat16 and bool(library().llmp_kv8_stream_supports(num_heads, num_kv_heads, head_dim, page_size))
 
 
-_kv8_sizes: Optional[Tuple[int, int]] = None     # floats of scratch and counters of a launch of the streaming kernel
-_kv8_counters: dict = {}
+@functools.lru_cache(maxsize=None)
+def _kv8_stream_sizes() -> Tuple[int, int]:
+    """Floats of scratch and counters that a launch of the streaming kernel needs."""
+    fn = library().llmp_kv8_stream_scratch_floats
+    fn.restype = _L
+    return int(fn()), int(library().llmp_kv8_stream_counters())
+
+
+_kv8_workspaces: dict = {}
 KV8_CAPTURED_CALLS = 4096                        # captured calls with counters from the slab
 
 
-def kv8_counters(device: torch.device, count: int) -> torch.Tensor:
-    """Zeroed counters for a launch of the streaming kernel, which leaves them zero. Calls on one stream follow one another
-    and share a set. A captured call gets a set of its own, since its graph may be replayed beside others: from a slab that was
-    made outside a capture, or, where there is none or it is used up, zeroed by the graph itself."""
-    key = device.index
+def kv8_workspace(device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Scratch and zeroed counters for a launch of the streaming kernel, which leaves the counters zero. Calls on one stream follow one
+    another and share a pair. A captured call gets a pair of its own, since its graph may be replayed beside others: counters from a
+    slab that was made outside a capture, or, where there is none or it is used up, counters that the graph itself zeroes."""
+    here = _device()
     if torch.cuda.is_current_stream_capturing():
-        slab = _kv8_counters.get((key, "slab"))
+        floats, count = _kv8_stream_sizes()
+        scratch = torch.empty(floats, dtype=torch.float32, device=device)
+        slab = _kv8_workspaces.get((here, "slab"))
         if slab is None or slab[1] + count > slab[0].numel():
-            return torch.zeros(count, dtype=torch.int32, device=device)
+            return scratch, torch.zeros(count, dtype=torch.int32, device=device)
         slab[1] += count
-        return slab[0][slab[1] - count:slab[1]]
-    counters = _kv8_counters.get((key, _stream()))
-    if counters is None:
-        counters = _kv8_counters[key, _stream()] = torch.zeros(count, dtype=torch.int32, device=device)
-        if (key, "slab") not in _kv8_counters:
-            _kv8_counters[key, "slab"] = [torch.zeros(KV8_CAPTURED_CALLS * count, dtype=torch.int32, device=device), 0]
-            torch.cuda.current_stream(device).synchronize()      # its captured users are ordered by nothing else
-    return counters
+        return scratch, slab[0][slab[1] - count:slab[1]]
+    pair = _kv8_workspaces.get((here, _stream()))
+    if pair is None:
+        floats, count = _kv8_stream_sizes()
+        pair = _kv8_workspaces[here, _stream()] = (torch.empty(floats, dtype=torch.float32, device=device),
+                                                   torch.zeros(count, dtype=torch.int32, device=device))
+        if (here, "slab") not in _kv8_workspaces:
+            _kv8_workspaces[here, "slab"] = [torch.zeros(KV8_CAPTURED_CALLS * count, dtype=torch.int32, device=device), 0]
+            torch.cuda.current_stream().synchronize()            # nothing else orders the zeros before a replay on another stream
+    return pair
 
 
 def kv8_decode_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, pages: torch.Tensor, block_tables: torch.Tensor,
@@ -2402,30 +2428,31 @@ def kv8_decode_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
     _kv8_pages(pages, num_kv_heads, head_dim, page_size)
     _i32(block_tables, "block_tables")
     _i32(ctx_len, "ctx_len")
-    R = ctx_len.numel()
-    _need(num_heads > 0 and num_heads % num_kv_heads == 0, f"{num_heads} query heads cannot share {num_kv_heads} key/value heads")
-    _need(q.dtype == out.dtype and q.dim() == 2 and q.shape[0] >= R and q.shape[1] >= num_heads * head_dim and q.stride(1) == 1 and
-          (R <= 1 or q.stride(0) == q_stride), "query rows must be [requests, at least heads * head_dim] of the output's type")
-    _need(out.is_contiguous() and out.shape == (R, num_heads * head_dim), "decode output must be [requests, heads * head_dim]")
-    _need(block_tables.dim() == 2 and block_tables.shape[0] == R and block_tables.shape[1] > 0, "block tables must be [requests, pages]")
-    _need(max_ctx > 0 and window >= 0, "the longest context must be positive, a window not negative")
-    _on_current_device(q, out, pages, block_tables, ctx_len)
+    R, width = ctx_len.numel(), num_heads * head_dim
+    if num_heads <= 0 or num_heads % num_kv_heads:
+        raise KernelError(f"{num_heads} query heads cannot share {num_kv_heads} key/value heads")
+    if not (q.dtype == out.dtype and q.dim() == 2 and q.shape[0] >= R and q.shape[1] >= width and q.stride(1) == 1 and
+            (R <= 1 or q.stride(0) == q_stride)):
+        raise KernelError("query rows must be [requests, at least heads * head_dim] of the output's type")
+    if not (out.is_contiguous() and out.shape == (R, width)):
+        raise KernelError("decode output must be [requests, heads * head_dim]")
+    if not (block_tables.dim() == 2 and block_tables.shape[0] == R and block_tables.shape[1] > 0):
+        raise KernelError("block tables must be [requests, pages]")
+    if max_ctx <= 0 or window < 0:
+        raise KernelError("the longest context must be positive, a window not negative")
     dtype = dtype_code(q.dtype)
-    if kv8_stream_supports(q.dtype, num_heads, num_kv_heads, head_dim, page_size) and (q.data_ptr() | 2 * int(q_stride)) % 16 == 0:
-        global _kv8_sizes
-        if _kv8_sizes is None:
-            fn = library().llmp_kv8_stream_scratch_floats
-            fn.restype = _L
-            _kv8_sizes = int(fn()), int(library().llmp_kv8_stream_counters())
-        scratch = torch.empty(_kv8_sizes[0], dtype=torch.float32, device=q.device)
-        _call("llmp_kv8_stream", _ptr(q), int(q_stride), _ptr(out), out.stride(0), _ptr(pages), pages.shape[0], _ptr(block_tables),
-              block_tables.shape[1], _ptr(ctx_len), R, int(max_ctx), num_heads, num_kv_heads, page_size, int(window), float(scale), _ptr(scratch),
-              _kv8_sizes[0], _ptr(kv8_counters(q.device, _kv8_sizes[1])), error_flag().data_ptr(), _stream())
+    _on_current_device(q, out, pages, block_tables, ctx_len)
+    at = q.data_ptr()
+    if kv8_stream_supports(q.dtype, num_heads, num_kv_heads, head_dim, page_size) and (at | 2 * q_stride) % 16 == 0 and out.data_ptr() % 8 == 0:
+        scratch, counters = kv8_workspace(q.device)
+        _call("llmp_kv8_stream", at, q_stride, out.data_ptr(), width, pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
+              block_tables.shape[1], ctx_len.data_ptr(), R, max_ctx, num_heads, num_kv_heads, page_size, window, scale, scratch.data_ptr(),
+              scratch.numel(), counters.data_ptr(), error_flag().data_ptr(), _stream())
         return out
     scratch = torch.empty(kv8_decode_scratch_floats(R, num_heads, head_dim, max_ctx), dtype=torch.float32, device=q.device)
-    _call("llmp_kv8_decode", _ptr(q), int(q_stride), _ptr(out), out.stride(0), dtype, _ptr(pages), pages.shape[0],
-          _ptr(block_tables), block_tables.shape[1], _ptr(ctx_len), R, int(max_ctx), num_heads, num_kv_heads, head_dim, page_size,
-          int(window), float(scale), _ptr(scratch), scratch.numel(), _stream())
+    _call("llmp_kv8_decode", at, q_stride, out.data_ptr(), width, dtype, pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
+          block_tables.shape[1], ctx_len.data_ptr(), R, max_ctx, num_heads, num_kv_heads, head_dim, page_size, window, scale, scratch.data_ptr(),
+          scratch.numel(), _stream())
     return out
 
 
@@ -2433,23 +2460,38 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     """tensor[dst[i]] = tensor[src[i]] for every i in each of the ``tensors`` (contiguous, one size of page, as many pages at
     least as the numbers ask for), in one launch for as many as its parameters take. No destination may be a source or twice
     a destination: the copies have no order."""
-    tensors, src, dst = list(tensors), [int(p) for p in src], [int(p) for p in dst]
-    _need(len(src) == len(dst), "as many destinations as sources are needed")
-    if not tensors or not src:
+    if len(src) != len(dst):
+        raise KernelError("as many destinations as sources are needed")
+    if not len(tensors) or not len(src):
         return
+    pairs = np.array([src, dst], dtype=np.int32)
     first = tensors[0]
-    _need(all(t.dim() >= 1 and t.is_contiguous() and t.dtype == first.dtype and t.shape[1:] == first.shape[1:] and t.device == first.device
-              for t in tensors), "the caches of a copy must be contiguous, of one page size, one type and on one device")
-    pages = min(t.shape[0] for t in tensors)
-    _need(all(0 <= p < pages for p in src) and all(0 <= p < pages for p in dst), f"a page to copy is outside 0..{pages - 1}")
-    _need(len(set(dst)) == len(dst) and not set(dst) & set(src), "a page is twice a destination, or a source and a destination")
-    _on_current_device(first)
-    page_bytes = first[0].numel() * first.element_size()
-    lib = library()
-    most_tensors, most_pairs = lib.llmp_copy_pages_max_tensors(), lib.llmp_copy_pages_max_pairs()
-    pointers = [_ptr(t) for t in tensors]
+    shape, kind = first.shape[1:], first.dtype
+    pages = first.shape[0] if first.dim() else 0
+    for t in tensors:
+        if not (t.dim() >= 1 and t.is_contiguous() and t.dtype == kind and t.shape[1:] == shape):
+            raise KernelError("the caches of a copy must be contiguous, of one page size and one type")
+        if t.shape[0] < pages:
+            pages = t.shape[0]
+    if int(pairs.min()) < 0 or int(pairs.max()) >= pages:
+        raise KernelError(f"a page to copy is outside 0..{pages - 1}")
+    role = np.zeros(pages, dtype=np.int32)                       # 1 per time a page is a destination, and a source
+    np.add.at(role, pairs[1], 1)
+    role[pairs[0]] += 1
+    if int(role[pairs[1]].max()) > 1:
+        raise KernelError("a page is twice a destination, or a source and a destination")
+    _on_current_device(*tensors)
+    page_bytes = math.prod(shape) * first.element_size()
+    most_tensors, most_pairs = _copy_pages_sizes()
+    pointers = [t.data_ptr() for t in tensors]
     for at in range(0, len(pointers), most_tensors):
         bases = (_P * len(pointers[at:at + most_tensors]))(*pointers[at:at + most_tensors])
         for i in range(0, len(src), most_pairs):
-            n = len(src[i:i + most_pairs])
-            _call("llmp_copy_pages", bases, len(bases), page_bytes, (_I * n)(*src[i:i + n]), (_I * n)(*dst[i:i + n]), n, _stream())
+            n = min(most_pairs, len(src) - i)
+            _call("llmp_copy_pages", bases, len(bases), page_bytes, pairs.ctypes.data + 4 * i, pairs.ctypes.data + 4 * (len(src) + i), n, _stream())
+
+
+@functools.lru_cache(maxsize=None)
+def _copy_pages_sizes() -> Tuple[int, int]:
+    """Caches and pages that one launch takes."""
+    return int(library().llmp_copy_pages_max_tensors()), int(library().llmp_copy_pages_max_pairs())
