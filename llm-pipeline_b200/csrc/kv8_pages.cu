@@ -4,7 +4,7 @@
 #define KV8_WARPS 4
 
 // ---- storing -----------------------------------------------------------------------------------------------------------
-// Rows of k and v [tokens, nkv * d] go to their slots (page * page_size + offset; negative: nowhere). A run is the
+// Rows of k and v [tokens, nkv * d] go to their slots (page * page_size + offset; negative or beyond the pages: nowhere). A run is the
 // consecutive rows of one page (rows without a slot between them aside). Per run and block (keys or values of one head):
 //   need = smallest scale that holds the run's largest finite magnitude
 //   e    = need, or the block's scale where that is larger and the run begins behind the page's first token
@@ -12,6 +12,11 @@
 //   the run's values:  q <- nearest(x * 2^(127 - e)), infinities and NaN to "no number"
 // One warp owns a run of a block, so nothing is shared; rows of one page that are not neighbours would be two runs that
 // write the same block at once. What lies behind the run in its page stays as it is.
+//
+// Latency bounds it (a warp has 4 KB to read and 2 KB to write): a warp reads the slots of its rows side by side and finds the runs
+// that begin among them by votes, and asks for a whole page of 16 tokens at once, which stays in registers from the search for the
+// largest to the rounding. 2,478 rows of 8 heads: 40 us with slots and rows read one after another, 13 so
+// (ncu, cold caches).
 struct StoreParams {
     const void* k;
     const void* v;
@@ -21,24 +26,45 @@ struct StoreParams {
     int N, nkv, d, page_size, num_pages, rows_per_block, wide;
 };
 
-template <typename T> __device__ __forceinline__ void kv8_load4(const T* p, int wide, float (&x)[4]) {
-    if (wide) {
-        if (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(p);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        } else {
-            const uint2 a = *reinterpret_cast<const uint2*>(p);
-            x[0] = __uint_as_float(a.x << 16); x[1] = __uint_as_float(a.x & 0xffff0000u);
-            x[2] = __uint_as_float(a.y << 16); x[3] = __uint_as_float(a.y & 0xffff0000u);
-        }
-    } else {
+// Eight entries of a row, as they lie there. `wide`: they start on 16 bytes.
+template <typename T> struct Eight {
+    uint4 raw[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p, int wide) {
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = to_float(p[i]);
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(raw)[i] = p[i];
+        }
     }
-}
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ float at(int i) const {
+        const unsigned w = reinterpret_cast<const unsigned*>(raw)[sizeof(T) == 4 ? i : i >> 1];
+        return __uint_as_float(sizeof(T) == 4 ? w : (i & 1 ? w & 0xffff0000u : w << 16));
+    }
+    __device__ __forceinline__ float largest(float amax) const {         // of the finite ones
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = fabsf(at(i));
+            if (a < INFINITY) amax = fmaxf(amax, a);
+        }
+        return amax;
+    }
+    __device__ __forceinline__ uint2 round(float up) const {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fabsf(at(i)) < INFINITY ? at(i) * up : __int_as_float(0x7fffffff);
+        return make_uint2(kv8_pack4(x[0], x[1], x[2], x[3]), kv8_pack4(x[4], x[5], x[6], x[7]));
+    }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_store_kernel(const StoreParams p) {
+    constexpr int HELD = 8;                                      // pieces of eight entries a lane holds: 16 tokens of 128 entries a warp
     pdl_trigger();
     pdl_wait();                                                  // the rows, and what the pages hold, are complete
     const int lane = threadIdx.x & 31;
@@ -47,69 +73,108 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_store_kernel(const StorePa
     const bool values = unit >= p.nkv;
     const T* src = reinterpret_cast<const T*>(values ? p.v : p.k) + (size_t)(values ? unit - p.nkv : unit) * p.d;
     const size_t stride = values ? p.v_stride : p.k_stride;
-    const int slots_end = p.num_pages * p.page_size, quads = p.d / 4;
-    auto slot_of = [&](int row) {                                // no slot beyond the pages is written to
-        const int s = p.slots[row];
+    const int slots_end = p.num_pages * p.page_size, pieces = p.d / 8;
+    auto slot_of = [&](int row) {
+        const int s = row < p.N ? p.slots[row] : -1;
         return s < slots_end ? s : -1;
     };
-    const int row_end = min(p.N, (int)(blockIdx.x + 1) * p.rows_per_block);
-    for (int first = blockIdx.x * p.rows_per_block; first < row_end; ++first) {
-        const int slot = slot_of(first);
-        if (slot < 0) continue;
-        const int page = slot / p.page_size;
-        int before = first - 1;
-        while (before >= 0 && slot_of(before) < 0) --before;
-        if (before >= 0 && slot_of(before) / p.page_size == page) continue;      // in the middle of a run
-        int end = first + 1, lowest = slot % p.page_size;
-        for (; end < p.N; ++end) {
-            const int s = slot_of(end);
-            if (s < 0) continue;
-            if (s / p.page_size != page) break;
-            lowest = min(lowest, s % p.page_size);
+    // the runs that begin among this block's rows
+    const int base = blockIdx.x * p.rows_per_block, window = min(p.rows_per_block, p.N - base);
+    const int slot = lane < window ? slot_of(base + lane) : -1;
+    const int page_here = slot < 0 ? -1 : slot / p.page_size;
+    const unsigned live = __ballot_sync(0xffffffffu, slot >= 0);
+    const unsigned lower = live & ((1u << lane) - 1u);
+    int page_before = __shfl_sync(0xffffffffu, page_here, lower ? 31 - __clz(lower) : 0);
+    if (slot >= 0 && !lower) {                                   // the first of them: the last row before the block that has a slot
+        int row = base - 1, s = -1;
+        for (; row >= 0 && (s = slot_of(row)) < 0; --row) {}
+        page_before = s < 0 ? -1 : s / p.page_size;
+    }
+    for (unsigned starts = __ballot_sync(0xffffffffu, slot >= 0 && page_before != page_here); starts; starts &= starts - 1u) {
+        const int begin = __ffs(starts) - 1;
+        const int page = __shfl_sync(0xffffffffu, page_here, begin), first = base + begin;
+        // the run's end, the lowest of its offsets, and whether they ascend (no slot twice)
+        int end = first, lowest = p.page_size, last = -1;
+        bool ordered = true;
+        for (bool more = true; more;) {
+            const int s = slot_of(end + lane);
+            const bool other = end + lane >= p.N || (s >= 0 && s / p.page_size != page);
+            const unsigned stop = __ballot_sync(0xffffffffu, other);
+            const int count = stop ? __ffs(stop) - 1 : 32;
+            const bool in = lane < count && s >= 0;
+            if (in) lowest = min(lowest, s % p.page_size);
+            const unsigned ins = __ballot_sync(0xffffffffu, in), lower = ins & ((1u << lane) - 1u);
+            const int before = __shfl_sync(0xffffffffu, s, lower ? 31 - __clz(lower) : 0);
+            if (in && s <= (lower ? before : last)) ordered = false;
+            if (ins) last = __shfl_sync(0xffffffffu, s, 31 - __clz(ins));
+            end += count;
+            more = !stop;
         }
+        lowest = __reduce_min_sync(0xffffffffu, lowest);
+        ordered = __all_sync(0xffffffffu, ordered);
         unsigned char* block = p.pages + (size_t)page * p.page_bytes + (size_t)unit * p.page_size * p.d;
         unsigned char* scale = p.pages + (size_t)page * p.page_bytes + (size_t)2 * p.nkv * p.page_size * p.d + unit;
-        const int count = (end - first) * quads;
+        const int count = (end - first) * pieces;
+        const int old = lowest > 0 ? *scale : 0;
+        // piece i of the run: entries 8 (i mod pieces) .. of its row i / pieces
+        Eight<T> held[HELD];
+        int to[HELD];                                            // where in the block it goes; -1: nowhere
+        auto ask = [&](int i, Eight<T>& x) {
+            x.none();
+            if (i >= count) return -1;
+            const int row = first + i / pieces, c = i % pieces * 8;
+            const int s = slot_of(row);
+            if (s < 0) return -1;
+            x.load(src + (size_t)row * stride + c, p.wide);
+            return s % p.page_size * p.d + c;
+        };
         float amax = 0.f;
-        for (int i = lane; i < count; i += 32) {
-            const int row = first + i / quads;
-            if (slot_of(row) < 0) continue;
-            float x[4];
-            kv8_load4(src + (size_t)row * stride + (i % quads) * 4, p.wide, x);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float a = fabsf(x[c]);
-                if (a < INFINITY) amax = fmaxf(amax, a);         // neither infinities nor NaN
-            }
+        for (int j = 0; j < HELD; ++j) to[j] = ask(j * 32 + lane, held[j]);
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) amax = held[j].largest(amax);
+        for (int i = HELD * 32 + lane; i < count; i += 32) {
+            Eight<T> x;
+            ask(i, x);
+            amax = x.largest(amax);
         }
         amax = warp_max(amax);
         int e = kv8_needed(amax);
-        if (lowest > 0) {
-            const int old = *scale;
-            if (old >= e) {
-                e = old;
-            } else {                                             // the tokens before the run move to the larger scale
-                const float down = kv8_power(max(old - e, -126));
-                for (int i = lane; i < lowest * quads; i += 32) {
-                    unsigned* at = reinterpret_cast<unsigned*>(block) + i;
-                    float q[4];
-                    kv8_unpack4(*at, q);
-                    *at = kv8_pack4(q[0] * down, q[1] * down, q[2] * down, q[3] * down);
-                }
+        if (lowest > 0 && old >= e) {
+            e = old;
+        } else if (lowest > 0) {                                 // the tokens before the run move to the larger scale
+            const float down = kv8_power(max(old - e, -126));
+            for (int i = lane; i < lowest * pieces; i += 32) {
+                uint2* at = reinterpret_cast<uint2*>(block) + i;
+                const uint2 w = *at;
+                float a[4], b[4];
+                kv8_unpack4(w.x, a);
+                kv8_unpack4(w.y, b);
+                *at = make_uint2(kv8_pack4(a[0] * down, a[1] * down, a[2] * down, a[3] * down),
+                                 kv8_pack4(b[0] * down, b[1] * down, b[2] * down, b[3] * down));
             }
         }
         __syncwarp();
         if (lane == 0) *scale = (unsigned char)e;
         const float up = kv8_power(127 - e);
-        for (int i = lane; i < count; i += 32) {
-            const int row = first + i / quads, c = (i % quads) * 4;
-            const int s = slot_of(row);
-            if (s < 0) continue;
-            float x[4];
-            kv8_load4(src + (size_t)row * stride + c, p.wide, x);
+        if (!ordered) {                                          // row by row: of a slot's rows the last one stays
+            for (int row = first; row < end; ++row) {
+                for (int c = lane; c < pieces; c += 32) {
+                    Eight<T> x;
+                    const int at = ask((row - first) * pieces + c, x);
+                    if (at >= 0) *reinterpret_cast<uint2*>(block + at) = x.round(up);
+                }
+                __syncwarp();
+            }
+            continue;
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = fabsf(x[j]) < INFINITY ? x[j] * up : __int_as_float(0x7fffffff);
-            *reinterpret_cast<unsigned*>(block + (size_t)(s % p.page_size) * p.d + c) = kv8_pack4(x[0], x[1], x[2], x[3]);
+        for (int j = 0; j < HELD; ++j)
+            if (to[j] >= 0) *reinterpret_cast<uint2*>(block + to[j]) = held[j].round(up);
+        for (int i = HELD * 32 + lane; i < count; i += 32) {
+            Eight<T> x;
+            const int at = ask(i, x);
+            if (at >= 0) *reinterpret_cast<uint2*>(block + at) = x.round(up);
         }
     }
 }
@@ -131,9 +196,9 @@ LLMP_API int llmp_kv8_store(const void* k, long k_stride, const void* v, long v_
     StoreParams p;
     p.k = k; p.v = v; p.slots = slots; p.pages = (unsigned char*)pages; p.k_stride = k_stride; p.v_stride = v_stride;
     p.page_bytes = kv8_page_bytes(nkv, page_size, d); p.N = N; p.nkv = nkv; p.d = d; p.page_size = page_size; p.num_pages = num_pages;
-    const size_t quad = dtype == LLMP_F32 ? 16 : 8;
-    p.wide = ((size_t)k % quad) == 0 && ((size_t)v % quad) == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
-    p.rows_per_block = N <= 256 ? 1 : 16;
+    const long row16 = dtype == LLMP_F32 ? 4 : 8;                // entries of 16 bytes
+    p.wide = ((size_t)k % 16) == 0 && ((size_t)v % 16) == 0 && k_stride % row16 == 0 && v_stride % row16 == 0;
+    p.rows_per_block = N <= 256 ? 1 : 16;                        // few rows: mostly single tokens, a run each
     const dim3 grid((N + p.rows_per_block - 1) / p.rows_per_block, (2 * nkv + KV8_WARPS - 1) / KV8_WARPS);
     LLMP_REQUIRE(grid.y <= 65535, "kv8_store: too many heads");
     if (dtype == LLMP_F32) llmp_launch_dependent(kv8_store_kernel<float>, grid, dim3(KV8_WARPS * 32), 0, stream, p);

@@ -153,6 +153,19 @@ def test_gather_is_exact_and_zeros_what_is_not_there(dtype, nkv, d, ps):
     assert torch.equal(out.double().cpu(), want)
 
 
+@pytest.mark.parametrize("d,ps", [(16, 64), (128, 16), (256, 8)])
+def test_store_of_slots_twice_and_out_of_order_keeps_the_last_row(d, ps):
+    gen = torch.Generator().manual_seed(8)
+    host = filled(3, 1, ps, d, 9)
+    pages = host.raw.to(DEV)
+    slots = [ps + 2, ps + 1, ps + 5, ps + 5, ps + 1, ps + 3] + [-1] * 40 + [ps + 5, ps + 2] + [s for s in range(2 * ps, 3 * ps)] + [3 * ps - 1]
+    x = torch.randn(len(slots), 2 * d, generator=gen)
+    host.store(x[:, :d], x[:, d:], slots)
+    on = x.to(DEV)
+    K().kv8_store(on[:, :d], on[:, d:], torch.tensor(slots, dtype=torch.int32, device=DEV), pages, 1, d, ps)
+    same_bytes(pages, host.raw)
+
+
 # ---- attention -----------------------------------------------------------------------------------------------------------
 
 def scattered(ctx, ps, P, seed):
