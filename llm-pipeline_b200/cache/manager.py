@@ -13,7 +13,8 @@ page in every cache of the group (a tensor ``[num_pages, *spec.page_shape(page_s
 ``[num_pages, 2, kv_heads, page_size, head_dim]`` for keys and values). A group whose layers see only a window or a chunk of keys gives pages back as soon as no later token
 sees a key in them (but for the pages of the first tokens where the spec keeps those visible); its block table then holds -1 there. Beside the pages, every live
 request owns a *slot*: an index into per-cache state tensors of fixed size per request, zeroed
-when the slot is handed out.
+when the slot is handed out. A request can be forked (``fork``): what it has begun with is held by several requests
+from then on, a page at a time; only a page that is filled in part is copied, since somebody will write to it.
 """
 
 from __future__ import annotations
@@ -26,6 +27,12 @@ import torch
 from .spec import PagesSpec, StateSpec
 
 
+def copy_pages(tensors, src, dst) -> None:
+    from ..ops import kernels
+
+    kernels.copy_pages(tensors, src, dst)
+
+
 class CacheError(RuntimeError):
     pass
 
@@ -33,14 +40,14 @@ class CacheError(RuntimeError):
 class PagePool:
     """Page ids 0..n-1 with a LIFO free list: the pages freed last are handed out first (in the order
     in which their holder held them), so reuse happens early and deterministically. Double frees and
-    foreign ids are errors."""
+    foreign ids are errors. A page may have several holders (``share``); it is free when each has freed it."""
 
     def __init__(self, num_pages: int):
         if num_pages <= 0:
             raise CacheError(f"a page pool needs at least one page, got {num_pages}")
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
-        self._is_free = [True] * num_pages
+        self._holders = [0] * num_pages
         self.high_water = 0
 
     @property
@@ -59,22 +66,47 @@ class PagePool:
             return None
         pages = [self._free.pop() for _ in range(n)]
         for p in pages:
-            self._is_free[p] = False
+            self._holders[p] = 1
         self.high_water = max(self.high_water, self.num_used)
         return pages
+
+    def holders(self, page: int) -> int:
+        return self._holders[page]
+
+    def share(self, pages: Sequence[int]) -> None:
+        """One more holder for each of the pages."""
+        for p in pages:
+            if not 0 <= p < self.num_pages or self._holders[p] == 0:
+                raise CacheError(f"page {p} is nobody's and cannot be shared")
+        for p in pages:
+            self._holders[p] += 1
 
     def free(self, pages: Sequence[int]) -> None:
         for p in pages:
             if not 0 <= p < self.num_pages:
                 raise CacheError(f"page {p} does not belong to this pool")
-            if self._is_free[p]:
+            if self._holders[p] == 0:
                 raise CacheError(f"page {p} freed twice")
         # In reverse, so that the pages of a run come out again in the order in which they were held: a request that
         # gets the pages of one that ended holds ascending ids again, and the attention kernels bring pages whose ids
         # follow one another in one TMA box.
         for p in reversed(pages):
-            self._is_free[p] = True
-            self._free.append(p)
+            if self._holders[p] == 0:
+                raise CacheError(f"page {p} freed twice")
+            self._holders[p] -= 1
+            if self._holders[p] == 0:
+                self._free.append(p)
+
+    def compact(self) -> Dict[int, int]:
+        """Moves the used pages to the lowest ids, as few as possible: {old id: new id}. The free pages are handed out in
+        ascending order after that. The caller copies what the pages hold and renames them wherever it keeps them."""
+        used = self.num_used
+        holes = [p for p in range(used) if self._holders[p] == 0]
+        moved = dict(zip((p for p in range(used, self.num_pages) if self._holders[p]), holes))
+        for old, new in moved.items():
+            self._holders[new], self._holders[old] = self._holders[old], 0
+        self._free = list(range(self.num_pages - 1, used - 1, -1))
+        return moved
 
     def free_ids(self) -> List[int]:
         return list(self._free)
@@ -263,6 +295,82 @@ class CacheManager:
             group.pool.free([p for p in table if p >= 0])
         self._free_slots.append(request.slot)
 
+    # -- copies ------------------------------------------------------------------------------
+    def fork(self, req_id: Hashable, new_ids: Sequence[Hashable], length: Optional[int] = None) -> bool:
+        """Requests ``new_ids`` that begin with the first ``length`` tokens of a live one (None: all it has): they hold its full
+        pages with it, copies of the page that is filled in part, and copies of its state. All or nothing; False when slots
+        or pages are too few. A request with state can only be forked at its present length, one whose window has moved on not before
+        what the window still holds. The copies are queued behind the steps that are issued, on the current stream."""
+        if req_id not in self._requests:
+            raise CacheError(f"request {req_id!r} is not live")
+        parent, new_ids = self._requests[req_id], list(new_ids)
+        length = parent.length if length is None else int(length)
+        if not 0 <= length <= parent.length:
+            raise CacheError(f"request {req_id!r} holds {parent.length} tokens and cannot be forked at {length}")
+        if self.state_specs and length != parent.length:
+            raise CacheError(f"request {req_id!r} has state of {parent.length} tokens and cannot be forked at {length}")
+        if len(set(new_ids)) != len(new_ids) or any(i in self._requests for i in new_ids):
+            raise CacheError("a fork needs new request ids")
+        full, part = divmod(length, self.page_size)
+        for group in self.groups:
+            table = group.tables[req_id]
+            if any(p < 0 for p in table[self._first_needed_page(group, length):full + (part > 0)]):
+                return False
+        need = len(new_ids) if part else 0
+        if len(new_ids) > len(self._free_slots) or any(need > group.pool.num_free for group in self.groups):
+            return False
+        slots = []
+        for new_id in new_ids:
+            slots.append(self._free_slots.pop())
+            self._admissions += 1
+            self._requests[new_id] = _Request(slots[-1], length, self._admissions)
+        for g, group in enumerate(self.groups):
+            table = group.tables[req_id]
+            copies = group.pool.alloc(need)
+            assert copies is not None
+            for new_id in new_ids:
+                group.pool.share([p for p in table[:full] if p >= 0])
+                group.tables[new_id] = table[:full]
+            for new_id, page in zip(new_ids, copies):
+                group.tables[new_id].append(page)
+                if page in self._ever_used[g]:
+                    self.pages_reused += 1
+                self._ever_used[g].add(page)
+            if copies and group.tensors:
+                copy_pages(list(group.tensors.values()), [table[full]] * need, copies)
+        for tensors in self._alike(self.states.values()):
+            if new_ids:
+                copy_pages(tensors, [parent.slot] * len(slots), slots)
+        return True
+
+    def compact(self) -> int:
+        """Move the pages in use to the lowest page ids, so that the free ones are one run at the end; returns how many
+        pages moved. Block tables that are remembered elsewhere are void: every request counts as newly admitted (``admission``)."""
+        total = 0
+        for g, group in enumerate(self.groups):
+            moved = group.pool.compact()
+            if not moved:
+                continue
+            total += len(moved)
+            for table in group.tables.values():
+                table[:] = [moved.get(p, p) for p in table]
+            self._ever_used[g].update(moved.values())
+            if group.tensors:
+                copy_pages(list(group.tensors.values()), list(moved), list(moved.values()))
+        if total:
+            for request in self._requests.values():
+                self._admissions += 1
+                request.admission = self._admissions
+        return total
+
+    @staticmethod
+    def _alike(tensors) -> List[List[torch.Tensor]]:
+        """The tensors in lists of one type and shape of a row."""
+        kinds: Dict[tuple, List[torch.Tensor]] = {}
+        for t in tensors:
+            kinds.setdefault((t.dtype, tuple(t.shape)), []).append(t)
+        return list(kinds.values())
+
     # -- views for the step function -------------------------------------------------------
     def pages_tensor(self, cache_id: int) -> torch.Tensor:
         return self.groups[self.group_of_cache[cache_id]].tensors[cache_id]
@@ -303,16 +411,16 @@ class CacheManager:
         }
 
     def check(self) -> None:
-        """Every page is either free or in exactly one block table; every slot likewise."""
+        """Every page is either free or in as many block tables as it has holders; every slot is free or one request's."""
         for g, group in enumerate(self.groups):
-            seen = {}
+            seen: Dict[int, List[Hashable]] = {}
             for req_id, table in group.tables.items():
                 for p in table:
-                    if p < 0:
-                        continue
-                    if p in seen:
-                        raise CacheError(f"group {g}: page {p} held by {seen[p]!r} and {req_id!r}")
-                    seen[p] = req_id
+                    if p >= 0:
+                        seen.setdefault(p, []).append(req_id)
+            for p, held_by in seen.items():
+                if len(set(held_by)) != len(held_by) or len(held_by) != group.pool.holders(p):
+                    raise CacheError(f"group {g}: page {p} held by {held_by!r}, its holders are {group.pool.holders(p)}")
             free = group.pool.free_ids()
             if len(set(free)) != len(free):
                 raise CacheError(f"group {g}: a page is twice in the free list")

@@ -28,7 +28,7 @@ def _cmd_infer(args: argparse.Namespace) -> int:
         model_path=args.model, device=args.device, dtype=args.dtype, max_new_tokens=args.max_new_tokens,
         temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, seed=args.seed,
         block_size=args.block_size, num_blocks=args.num_blocks, max_sequence_length=args.max_sequence_length,
-        max_num_batched_tokens=args.max_num_batched_tokens))
+        max_num_batched_tokens=args.max_num_batched_tokens, kv_cache_dtype=args.kv_cache_dtype))
     if args.prompt_ids is not None:
         prompt = [int(t) for t in args.prompt_ids.replace(",", " ").split()]
         out = engine.generate(prompt, max_tokens=args.max_new_tokens, temperature=args.temperature)
@@ -85,6 +85,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     p.add_argument("--num-blocks", type=int, default=None)
     p.add_argument("--max-sequence-length", type=int, default=2048)
     p.add_argument("--max-num-batched-tokens", type=int, default=2048)
+    p.add_argument("--kv-cache-dtype", default=None, choices=("e4m3",), help="hold keys and values in 8 bits with a scale per page and head")
     p.set_defaults(fn=_cmd_infer)
 
     p = sub.add_parser("random-model", help="Write a model folder with seeded random weights")

@@ -42,11 +42,13 @@ class GenerationEngine:
                  num_pages: Optional[int] = None, memory_fraction: float = 0.8, max_num_seqs: int = 64,
                  max_num_batched_tokens: int = 2048, max_model_len: Optional[int] = None,
                  max_prefill_chunk: Optional[int] = None, sampling: Optional[SamplingConfig] = None,
-                 lookahead: Optional[bool] = None):
+                 lookahead: Optional[bool] = None, kv_cache_dtype: Optional[str] = None):
+        """``kv_cache_dtype``: None to hold keys and values in the model's type, "e4m3" for 8 bits with a scale per page and head in
+        the layers of grouped-query attention (``Model.cache_specs``)."""
         self.model, self.config = model, config
         self.device, self.dtype = model.device, model.dtype
         max_model_len = int(max_model_len or model.spec.max_position)
-        specs = model.cache_specs()
+        self.cache_specs = specs = model.cache_specs(kv_cache_dtype)
         if num_pages is None:
             num_pages = self._pages_that_fit(specs, page_size, memory_fraction, max_num_seqs, max_model_len)
         self.cache = CacheManager(specs, page_size=page_size, num_pages=num_pages, max_requests=max_num_seqs,
@@ -57,6 +59,7 @@ class GenerationEngine:
         self._ids = itertools.count()
         self._requests: Dict[Hashable, Request] = {}
         self.lookahead = os.environ.get("LLMP_B200_LOOKAHEAD", "1") != "0" if lookahead is None else bool(lookahead)
+        self._forks: Dict[Hashable, List[Request]] = {}      # requests that are to begin with another one's prompt, by its id
         self._in_flight = None                   # (sampled ids on the device, their requests, their landing place) of the step not read back yet
         self._landing: list = []                 # pinned host buffers with an event each, for the sampled ids' way to the host
         self.steps = 0
@@ -82,9 +85,11 @@ class GenerationEngine:
     def add_request(self, prompt_token_ids: Sequence[int], max_tokens: int = 16,
                     sampling: Optional[SamplingConfig] = None, eos_token_ids: Optional[Sequence[int]] = None,
                     ignore_eos: bool = False, req_id: Optional[Hashable] = None,
-                    position_ids: Optional[Sequence[Sequence[int]]] = None) -> Hashable:
+                    position_ids: Optional[Sequence[Sequence[int]]] = None, same_prompt_as: Optional[Hashable] = None) -> Hashable:
         """``position_ids``: for a model whose position encoding reads several streams of positions, the prompt's
-        position ids, one sequence per stream (see ``Request.position_ids``)."""
+        position ids, one sequence per stream (see ``Request.position_ids``). ``same_prompt_as``: a request with this very prompt that
+        has not been read to its end yet: this one then shares its pages instead of computing the prompt again (where the
+        model has state per request, or slots or pages are short, it is computed again)."""
         req_id = next(self._ids) if req_id is None else req_id
         if req_id in self._requests and self._requests[req_id].status != "finished":
             raise ValueError(f"request id {req_id!r} is in use")
@@ -100,9 +105,42 @@ class GenerationEngine:
         request = Request(req_id, [int(t) for t in prompt_token_ids], sampling or self.sampler.config,
                           int(max_tokens), set(int(t) for t in eos_token_ids), ignore_eos,
                           position_ids=None if position_ids is None else [[int(x) for x in row] for row in position_ids])
+        if same_prompt_as is not None:
+            first = self._requests.get(same_prompt_as)
+            if first is None or first.prompt != request.prompt or first.position_ids != request.position_ids:
+                raise ValueError(f"request {same_prompt_as!r} is unknown or has another prompt")
+            if not self.cache.state_specs and first.computed < len(first.prompt) and first.status in ("waiting", "running"):
+                self.scheduler.check(request)
+                self._forks.setdefault(same_prompt_as, []).append(request)
+                self._requests[req_id] = request
+                return req_id
         self.scheduler.add(request)
         self._requests[req_id] = request
         return req_id
+
+    def _fork(self, plan: StepPlan) -> None:
+        """After a step was issued: the requests that wait for a prompt it has finished. They share all of it but its last token, which
+        they run again in the next step, for the logits that their own first token is sampled from. What cannot be
+        shared (no slot, no page, no room among the running requests) is computed like any other request."""
+        for entry in plan.entries:
+            first = entry.request
+            if first.req_id not in self._forks or entry.start + entry.count < len(first.prompt):
+                continue
+            waiting = self._forks.pop(first.req_id)
+            shared = len(first.prompt) - 1
+            room = min(len(waiting), self.scheduler.max_num_seqs - len(self.scheduler.running), self.cache.free_slots)
+            now = waiting[:max(room, 0)] if shared else []
+            if now and self.cache.fork(first.req_id, [r.req_id for r in now], shared):
+                for request in now:
+                    self.scheduler.add_forked(request, shared)
+                waiting = waiting[len(now):]
+            for request in waiting:
+                self.scheduler.add(request)
+
+    def _unfork(self, request: Request) -> None:
+        """The request ended before its prompt was computed: those that wait for it go their own way."""
+        for waiting in self._forks.pop(request.req_id, []):
+            self.scheduler.add(waiting)
 
     def has_unfinished(self) -> bool:
         # (ids still in flight for requests that are all finished, stopped or aborted meanwhile, are nobody's business)
@@ -127,6 +165,8 @@ class GenerationEngine:
         if not ahead:
             finished += self._read_back()
         plan: StepPlan = self.scheduler.schedule()
+        for request in plan.aborted:
+            self._unfork(request)
         finished += plan.aborted
         if not plan.entries:
             if self._in_flight is not None:
@@ -149,6 +189,8 @@ class GenerationEngine:
                     raise RuntimeError("a token that is still on the device can only be a step's single token")
             entries.append(StepEntry(e.request.req_id, tokens, [e.count - 1] if e.samples else [], e.positions, on_device))
         logits = self.runner.step(entries)
+        if self._forks:
+            self._fork(plan)
         due = [e for e in plan.entries if e.samples]
         launched = None
         if due:
@@ -178,7 +220,15 @@ class GenerationEngine:
 
     def abort(self, req_id: Hashable) -> Optional[Request]:
         """Take the request out wherever it is; its pages go back. What is still in flight for it is dropped."""
+        for first, waiting in self._forks.items():
+            for request in waiting:
+                if request.req_id == req_id:
+                    waiting.remove(request)
+                    request.status, request.finish_reason = "finished", "abort"
+                    return request
         request = self.scheduler.abort(req_id)
+        if request is not None:
+            self._unfork(request)
         if request is None:
             request = self._requests.get(req_id)
             if request is None or request.status != "draining":
@@ -209,14 +259,20 @@ class GenerationEngine:
     # -- whole generations -------------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], max_tokens: int = 16, temperature: Optional[float] = None,
                  top_k: Optional[int] = None, top_p: Optional[float] = None, seed: Optional[int] = None,
-                 ignore_eos: bool = False, **sampling_overrides) -> List[GenerationResult]:
+                 ignore_eos: bool = False, samples_per_prompt: int = 1, **sampling_overrides) -> List[GenerationResult]:
         """Generate for every prompt (lists of token ids); results in the order of the prompts.
-        Prompt i samples with seed ``seed + i``."""
+        Prompt i samples with seed ``seed + i``. ``samples_per_prompt`` = n: n results for every prompt, one after another,
+        with seeds ``seed + n i`` to ``seed + n i + n - 1``; the prompt is computed once and its pages are shared."""
+        if samples_per_prompt < 1:
+            raise ValueError("samples_per_prompt must be at least 1")
         base = self.sampler.config.merged({"temperature": temperature, "top_k": top_k, "top_p": top_p,
                                            **sampling_overrides})
         first_seed = base.seed if seed is None else int(seed)
-        ids = [self.add_request(p, max_tokens, replace(base, seed=first_seed + i), ignore_eos=ignore_eos)
-               for i, p in enumerate(prompts)]
+        ids = []
+        for i, p in enumerate(prompts):
+            for k in range(samples_per_prompt):
+                ids.append(self.add_request(p, max_tokens, replace(base, seed=first_seed + len(ids)), ignore_eos=ignore_eos,
+                                            same_prompt_as=ids[-k] if k else None))
         while any(self._requests[i].status != "finished" for i in ids):
             self.step()
         results = []

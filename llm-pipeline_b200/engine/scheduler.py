@@ -131,7 +131,7 @@ class Scheduler:
         self.num_finished = 0
 
     # -- requests --------------------------------------------------------------------------
-    def add(self, request: Request) -> None:
+    def check(self, request: Request) -> None:
         if not request.prompt:
             raise ValueError(f"request {request.req_id!r} has an empty prompt")
         if len(request.prompt) >= self.max_model_len:
@@ -139,8 +139,16 @@ class Scheduler:
                              f"to generate within {self.max_model_len} tokens")
         if request.max_tokens < 1:
             raise ValueError("max_tokens must be at least 1")
+
+    def add(self, request: Request) -> None:
+        self.check(request)
         request.status = "waiting"
         self.waiting.append(request)
+
+    def add_forked(self, request: Request, computed: int) -> None:
+        """A request whose first ``computed`` tokens the cache already holds (``CacheManager.fork``): it runs at once."""
+        request.status, request.computed = "running", computed
+        self.running.append(request)
 
     def has_unfinished(self) -> bool:
         return bool(self.waiting or self.running)

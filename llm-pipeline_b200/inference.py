@@ -56,6 +56,8 @@ class Qwen3InferenceConfig:
     # scheduler
     max_num_batched_tokens: int = 2048
     max_prefill_chunk: Optional[int] = None
+    # keys and values: None in the model's type, "e4m3" in 8 bits with a scale for each page and head
+    kv_cache_dtype: Optional[str] = None
 
 
 def resolve_dtype(dtype: Union[torch.dtype, str]) -> torch.dtype:
@@ -81,7 +83,7 @@ class Qwen3InferenceEngine:
             config.model_path, device=config.device, dtype=dtype, page_size=config.block_size,
             num_pages=config.num_blocks, memory_fraction=config.memory_fraction, max_num_seqs=config.max_batch_size,
             max_num_batched_tokens=config.max_num_batched_tokens, max_model_len=config.max_sequence_length,
-            max_prefill_chunk=config.max_prefill_chunk, sampling=sampling)
+            max_prefill_chunk=config.max_prefill_chunk, sampling=sampling, kv_cache_dtype=config.kv_cache_dtype)
         self.model_config = self.engine.config
         self._continuous: dict = {}              # add_continuous_request: id -> (prompt as given, time it was added)
         self._continuous_done: dict = {}         # id -> time its result was first seen finished
@@ -125,20 +127,26 @@ class Qwen3InferenceEngine:
             outs = [self.tokenizer.decode(r.token_ids, skip_special_tokens=True) for r in results]
         else:
             outs = [r.token_ids for r in results]
-        return outs[0] if single else outs
+        return outs[0] if single and len(outs) == 1 else outs
 
     def generate_ids(self, prompts: Sequence[Sequence[int]], max_tokens: Optional[int] = None,
                      temperature: Optional[float] = None, top_k: Optional[int] = None, top_p: Optional[float] = None,
-                     **kwargs) -> List[GenerationResult]:
+                     num_return_sequences: int = 1, **kwargs) -> List[GenerationResult]:
+        """``num_return_sequences`` = n: n results for every prompt, one after another, each sampled with a seed of its own; the
+        prompt is computed once and its pages are shared."""
+        if num_return_sequences < 1:
+            raise ValueError("num_return_sequences must be at least 1")
         max_tokens = max_tokens or self.config.max_new_tokens
         results: List[GenerationResult] = []
         prompts = list(prompts)
         eos = self._eos_ids()
         base = self.engine.sampler.config.merged({"temperature": temperature, "top_k": top_k, "top_p": top_p, **kwargs})
         from dataclasses import replace
-        ids = [self.engine.add_request(p, max_tokens, replace(base, seed=base.seed + i), eos_token_ids=eos,
-                                       ignore_eos=bool(kwargs.get("ignore_eos", False)))
-               for i, p in enumerate(prompts)]
+        ids = []
+        for p in prompts:
+            for k in range(num_return_sequences):
+                ids.append(self.engine.add_request(p, max_tokens, replace(base, seed=base.seed + len(ids)), eos_token_ids=eos,
+                                                   ignore_eos=bool(kwargs.get("ignore_eos", False)), same_prompt_as=ids[-k] if k else None))
         mine = [self.engine._requests[i] for i in ids]
         # until every request of THIS call is finished: requests of other callers (an open stream, add_request) may
         # finish meanwhile and are none of this call's business
@@ -286,12 +294,16 @@ class Qwen3InferenceEngine:
         memory_mb = info["total_parameters"] * bytes_per_param / (1024 * 1024)
         memory_gb = memory_mb / 1024
         from .cache import CacheManager
-        per_page = sum(CacheManager.bytes_per_page(self.engine.model.cache_specs(), self.engine.cache.page_size, self.engine.dtype))
+        per_page = sum(CacheManager.bytes_per_page(self.engine.cache_specs, self.engine.cache.page_size, self.engine.dtype))
         return {**{k: v for k, v in info.items() if k.endswith("parameters") or k.endswith("_per_layer")},
                 "memory_mb": memory_mb, "memory_gb": memory_gb, "model_memory_mb": memory_mb, "model_memory_gb": memory_gb,
                 "bytes_per_param": bytes_per_param, "dtype": str(self.engine.dtype),
                 "recommended_gpu_memory_gb": max(memory_gb * 1.5, memory_gb + 1.0),
                 "kv_cache_bytes_per_token": per_page // self.engine.cache.page_size}
+
+    def compact_kv_cache(self) -> int:
+        """Move the cache's pages in use together; returns how many moved (``CacheManager.compact``)."""
+        return self.engine.cache.compact()
 
     def cleanup(self) -> None:
         """Abort whatever is still queued or running and give its pages back."""
