@@ -1,0 +1,587 @@
+// Causal attention of prompt portions over pages of 8-bit keys and values (kv8.cuh) on the fifth-generation tensor cores: bfloat16
+// queries, head size 128, as llmp_paged_attention over pages of bfloat16.
+//
+// A block takes 256 query rows of one request and one key/value head (a row is a token and a query head of the group, the head running
+// fastest) as two tiles of 128, and walks tiles of 128 keys. All products are in half precision, which holds every e4m3 value exactly:
+//   unpack       four warps turn a tile's bytes into half precision, laid out as operands; both row tiles use what is unpacked once
+//   S = Q K^T    Q, K in shared memory (128-byte swizzle, K-major), S in tensor memory
+//   softmax      a thread has a row: it reads S from tensor memory twice, 32 columns at a time, and writes factors over S
+//   O += P V     P read from tensor memory, V in shared memory MN-major, O in tensor memory
+// While one row tile is in its softmax the tensor cores work for the other. The two tiles' S and O fill the tensor memory (512 columns).
+//
+// With t = log2(e) scale q.k and a value's scale 2^v, weights are 2^t and the factor of a value's bytes is 2^(t + v). As in
+// attention_decode_kv8_stream.cu each has its own maximum, m and mu, raised to a whole number when it is passed by more than 8: factors
+// are held in half precision relative to 2^mu, the sum l of the weights in float32 relative to 2^m, and out = O / l * 2^(mu - m). A
+// block of eight keys has one scale, so a weight is its factor times 2^(mu - m - v), a power of two; only where that is beyond 2^100 are
+// the weights computed apart. Queries are brought to a largest magnitude in [1, 4) by a power of two per row.
+//
+// What cannot be seen does not matter: values behind the context and in missing pages are zeros as operands; a value that is no number is
+// one too, and the rows that see its key become no number by their l.
+//
+// Roles: warps 0-3 and 4-7 softmax of the two row tiles, 8-11 unpacking, 12 loads (TMA, a page and head in a box, keys and values
+// together), 13 issues the products. Few rows over many keys: an item of the list is a part of a row tile's keys and leaves its sums
+// in global memory, and prompt_kv8_merge_kernel adds them up. Every wait on an mbarrier is bounded: when one runs out the kernel records
+// 1 in *error_flag and goes on without waiting (its output is then wrong; the host reads the flag).
+#include "kv8.cuh"
+#include "prefill_tc.cuh"
+#include "tcgen05.cuh"
+
+#define P8_D 128
+#define P8_ROWS 128                                  // of a row tile
+#define P8_KEYS 128
+#define P8_THREADS 448
+#define P8_HALF (P8_ROWS * 128)                      // bytes of 128 rows of 64 entries in half precision
+#define P8_RAW_STAGE (2 * P8_KEYS * P8_D)            // bytes of a tile's keys and values
+#define P8_SCALE_SLOTS 4                             // a tile's scales live until its softmax: at most four tiles are on their way
+#define P8_PART (P8_D + 4)                           // floats of a row's sums: O, m, mu, l
+
+struct Prompt8Params {
+    const bf16* q;
+    bf16* out;
+    const unsigned char* pages;
+    const int* block_tables;
+    const int* q_start;
+    const int* ctx_len;
+    const int* items;                                // [num_items][4]: request, first token, part | parts << 16, place of the item's sums
+    float* partials;                                 // [places][nkv][256][P8_PART]
+    long q_stride, out_stride, page_bytes;
+    int table_stride, num_pages, nq, nkv, page_size, page_shift, window, tokens;
+    float scale;
+    int* error_flag;
+};
+
+__device__ __forceinline__ void p8_load_box(void* smem_dst, const CUtensorMap* map, int token, int kvh, int page, uint64_t* bar) {
+    const int zero = 0;
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n"
+        ::"r"(tc_smem_u32(smem_dst)), "l"(map), "r"(tc_smem_u32(bar)), "r"(zero), "r"(token), "r"(kvh), "r"(zero), "r"(page) : "memory");
+}
+
+// Instruction descriptor of kind::f16 with half-precision operands and float32 sums, M x N.
+__host__ __device__ constexpr uint32_t p8_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+// Shared-memory descriptor of an MN-major operand in the 128-byte swizzle: rows of 64 contiguous entries, one per K index, eight of
+// them 1024 bytes, the next 64 entries P8_HALF further.
+__device__ __forceinline__ uint64_t p8_desc_mn(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(P8_HALF >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void p8_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(tc_smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ unsigned p8_half2(float lo, float hi) {
+    unsigned r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 2^n for whole numbers -126 <= n <= 127 in a float, by its bits.
+__device__ __forceinline__ float p8_power(float n) { return __int_as_float((__float_as_int(n + 12582912.f) + 127) << 23); }
+
+// The keys of a tile that one row sees are first .. last (in the tile); the scales of its blocks of eight keys.
+struct Tile8 {
+    const float2* scales;                            // of the 16 blocks: the keys' scale times nothing yet, the exponent of the values'; missing: 0, -inf
+    float f;                                         // log2(e) * scale * the query row's own power of two
+    int first, last;
+};
+
+// The largest t and t + v among 32 scores, of the tile's columns from `col` on.
+template <bool MASK>
+__device__ __forceinline__ void p8_top(const uint32_t (&x)[32], int col, const Tile8& tile, float& t_top, float& u_top) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const float2 s = tile.scales[col / 8 + b];
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = col + b * 8 + i;
+            const float v = __uint_as_float(x[b * 8 + i]);
+            if (!MASK || (key >= tile.first && key <= tile.last)) top = fmaxf(top, v);
+        }
+        const bool none = s.y == -INFINITY || (MASK && top == -INFINITY);
+        const float t = none ? -INFINITY : top * (s.x * tile.f);
+        t_top = fmaxf(t_top, t);
+        u_top = fmaxf(u_top, t + s.y);
+    }
+}
+
+// The factors of 32 scores as pairs in half precision; adds their weights to l.
+template <bool MASK>
+__device__ __forceinline__ void p8_factors(const uint32_t (&x)[32], int col, const Tile8& tile, float m, float mu, uint32_t (&pk)[16], float& l) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const float2 s = tile.scales[col / 8 + b];
+        const float c = s.x * tile.f, add = s.y - mu;
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = col + b * 8 + i;
+            p[i] = fa_ex2(fmaf(__uint_as_float(x[b * 8 + i]), c, add));
+            if (MASK && (key < tile.first || key > tile.last)) p[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pk[b * 4 + i] = p8_half2(p[2 * i], p[2 * i + 1]);
+        const float n = mu - m - s.y;                // weight = factor * 2^n
+        if (n <= 100.f) {
+            l = fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), p8_power(fmaxf(n, -126.f)), l);
+        } else if (s.y > -INFINITY) {                // factors too small for float32 although their weights are not
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = col + b * 8 + i;
+                if (!MASK || (key >= tile.first && key <= tile.last)) l += fa_ex2(fmaf(__uint_as_float(x[b * 8 + i]), c, -m));
+            }
+        }
+    }
+}
+
+template <int BOX>
+__global__ void __launch_bounds__(P8_THREADS, 1)
+prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p) {
+    extern __shared__ unsigned char p8_raw[];
+    __shared__ __align__(8) uint64_t raw_full[2], raw_free[2], k_full, k_free, v_full, v_free, s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(16) float2 scales[P8_SCALE_SLOTS][16];
+    __shared__ unsigned no_number[P8_SCALE_SLOTS][4];            // keys of a tile whose values hold NaN
+    __shared__ uint32_t tmem_slot;
+    const uint32_t raw_addr = tc_smem_u32(p8_raw);
+    unsigned char* Qs = p8_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);     // [2 tiles][2 halves][128 rows][128 bytes]
+    unsigned char* Ks = Qs + 4 * P8_HALF;                        // [2 halves][128 keys][128 bytes]
+    unsigned char* Vs = Ks + 2 * P8_HALF;
+    unsigned char* raw = Vs + 2 * P8_HALF;                       // [2 stages][box][keys, values][token][128 bytes]
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (warp == 12 && lane == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&raw_full[i], 2);                          // the boxes, and the scales
+            mbar_init(&raw_free[i], 4);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init(&k_full, 4);
+        mbar_init(&k_free, 1);
+        mbar_init(&v_full, 4);
+        mbar_init(&v_free, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
+    }
+    if (warp == 13) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    pdl_trigger();
+    pdl_wait();
+
+    // ---- what the item is ----
+    const int4 item = reinterpret_cast<const int4*>(p.items)[blockIdx.x / (unsigned)p.nkv];
+    const int kvh = (int)(blockIdx.x % (unsigned)p.nkv), r = item.x, tok0 = item.y, part = item.z & 0xffff, parts = item.z >> 16;
+    const int G = p.nq / p.nkv;
+    const int q_begin = p.q_start[r], q_len = p.q_start[r + 1] - q_begin;
+    const int ctx = min(p.ctx_len[r], p.table_stride << p.page_shift), pos0 = p.ctx_len[r] - q_len;
+    const int ntok = min(q_len - tok0, p.tokens);
+    const int rows = ntok * G;
+    const int* table = p.block_tables + (size_t)r * p.table_stride;
+    // keys of the whole row tile, and this part's tiles of them; a row tile of 128 rows sees none beyond its last row's position
+    const int low = p.window > 0 ? max(pos0 + tok0 - p.window + 1, 0) : 0;
+    const int tile0 = low / P8_KEYS, all_tiles = (pos0 + tok0 + ntok - 1) / P8_KEYS + 1 - tile0;
+    const int t_begin = tile0 + (int)((long)all_tiles * part / parts), t_end = tile0 + (int)((long)all_tiles * (part + 1) / parts);
+    int n[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int last_row = min(rows, (t + 1) * P8_ROWS) - 1;   // of the tile; below its first: the tile has no rows
+        n[t] = last_row < t * P8_ROWS ? 0 : max(min(t_end, (pos0 + tok0 + last_row / G) / P8_KEYS + 1) - t_begin, 0);
+    }
+    const int tiles = max(n[0], n[1]);
+
+    // ---- a softmax thread's row: its queries into shared memory ----
+    const int mine = warp >> 2, row = tid & (P8_ROWS - 1);       // row tile and row, of warps 0 .. 7
+    float f = 0.f;
+    if (warp < 8) {
+        const int index = mine * P8_ROWS + row;
+        uint4 v[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (index < rows) {
+            const uint4* q = reinterpret_cast<const uint4*>(p.q + (size_t)(q_begin + tok0 + index / G) * p.q_stride + (size_t)(kvh * G + index % G) * P8_D);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) v[c] = q[c];
+        }
+        float amax = 0.f;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            const unsigned w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+        }
+        int e = (int)(__float_as_uint(amax) >> 23);              // 2^(e - 127) <= amax < 2^(e - 126)
+        e = e < 1 ? 1 : (e > 253 ? 253 : e);
+        const float down = kv8_power(127 - e);
+        f = p.scale * 1.4426950408889634f * kv8_power(e - 127);
+        unsigned char* to = Qs + (size_t)mine * 2 * P8_HALF + row * 128;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            const unsigned w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+            unsigned h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = p8_half2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
+            *reinterpret_cast<uint4*>(to + (c >> 3) * P8_HALF + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    }
+    fa_fence_before();
+    __syncthreads();
+    fa_fence_after();
+    const uint32_t tmem = tmem_slot;                             // S of the tiles in columns 0 and 128, O in 256 and 384
+
+    if (warp == 12) {
+        // ---- loads: lane b < 16 sees to block b of eight keys; page numbers two tiles ahead, scale bytes one ----
+        const bool boxes = lane < 16 && (lane * 8) % BOX == 0;
+        const size_t body = (size_t)2 * p.nkv * p.page_size * P8_D;
+        auto find = [&](int j) {
+            const int key = (t_begin + j) * P8_KEYS + lane * 8;
+            return j < tiles && lane < 16 && key < ctx ? table[key >> p.page_shift] : -1;
+        };
+        unsigned ek = 0u, ev = 0u;
+        auto ask = [&](int& page) {
+            if (page >= p.num_pages) page = -1;
+            if (page >= 0) {
+                const unsigned char* at = p.pages + (size_t)page * p.page_bytes + body + kvh;
+                ek = at[0];
+                ev = at[p.nkv];
+            }
+        };
+        int now = find(0), next = find(1);
+        ask(now);
+        for (int j = 0; j < tiles; ++j) {
+            const int after = find(j + 2), stage = j & 1;
+            if (j > 1) mbar_wait(&raw_free[stage], ((j >> 1) - 1) & 1, p.error_flag);
+            if (lane == 0) mbar_expect_tx(&raw_full[stage], P8_RAW_STAGE);
+            __syncwarp();
+            if (boxes)                                           // out of range: the box arrives as zeros
+                p8_load_box(raw + stage * P8_RAW_STAGE + lane * 8 * 2 * P8_D, &map, ((t_begin + j) * P8_KEYS + lane * 8) & (p.page_size - 1), kvh,
+                            now >= 0 ? now : p.num_pages, &raw_full[stage]);
+            if (lane < 16) scales[j % P8_SCALE_SLOTS][lane] = now >= 0 ? make_float2(kv8_scale(ek), (float)((int)ev - 127)) : make_float2(0.f, -INFINITY);
+            __syncwarp();
+            if (lane == 0) p8_arrive(&raw_full[stage]);
+            now = next;
+            next = after;
+            ask(now);
+        }
+    } else if (warp == 13) {
+        // ---- products ----
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = p8_idesc(P8_ROWS, P8_KEYS), idesc_o = p8_idesc(P8_ROWS, P8_D) | (1u << 16);      // V is MN-major
+            const uint32_t q_addr = tc_smem_u32(Qs), k_addr = tc_smem_u32(Ks), v_addr = tc_smem_u32(Vs);
+            const int last_t = n[1] > 0 ? 1 : 0;
+            // S of row tile t and key tile j; the first of the row tiles waits for the keys, the last frees them
+            auto scores = [&](int t, int j) {
+                if (t == 0 || j >= n[0]) mbar_wait(&k_full, j & 1, p.error_flag);
+                fa_fence_after();
+#pragma unroll
+                for (int k = 0; k < P8_D / 16; ++k) {
+                    const uint32_t off = (uint32_t)(k >> 2) * P8_HALF + (uint32_t)(k & 3) * 32;
+                    umma_f16(tmem + t * 128, umma_desc(q_addr + t * 2 * P8_HALF + off), umma_desc(k_addr + off), idesc_s, k != 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[t]);
+                if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&k_free);
+            };
+            for (int t = 0; t < 2; ++t)
+                if (n[t] > 0) scores(t, 0);
+            for (int j = 0; j < tiles; ++j) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (j >= n[t]) continue;
+                    mbar_wait(&p_full[t], j & 1, p.error_flag);
+                    if (t == 0 || j >= n[0]) mbar_wait(&v_full, j & 1, p.error_flag);
+                    fa_fence_after();
+#pragma unroll
+                    for (int k = 0; k < P8_KEYS / 16; ++k)       // 16 keys a product: 8 columns of P, 2 KB of V
+                        fa_umma_a_tmem(tmem + 256 + t * 128, tmem + t * 128 + k * 8, p8_desc_mn(v_addr + k * 2048), idesc_o, (j | k) != 0 ? 1u : 0u);
+                    umma_commit(&o_done[t]);
+                    if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&v_free);
+                    if (j + 1 < n[t]) scores(t, j + 1);
+                }
+            }
+        }
+    } else if (warp >= 8) {
+        // ---- unpacking: a thread has a key ----
+        const int key = tid - 256;
+        const int from = (key / BOX) * 2 * BOX * P8_D + (key % BOX) * P8_D, to = key * 128;
+        for (int j = 0; j < tiles; ++j) {
+            const unsigned char* src = raw + (j & 1) * P8_RAW_STAGE + from;
+            mbar_wait(&raw_full[j & 1], (j >> 1) & 1, p.error_flag);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                if (j > 0) mbar_wait(kv == 0 ? &k_free : &v_free, (j - 1) & 1, p.error_flag);
+                unsigned char* dst = (kv == 0 ? Ks : Vs) + to;
+                // what is not there as zeros: it meets factors of zero
+                const bool there = kv == 0 || ((t_begin + j) * P8_KEYS + key < ctx && scales[j % P8_SCALE_SLOTS][key / 8].y > -INFINITY);
+                bool nan = false;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint4 four = *reinterpret_cast<const uint4*>(src + kv * BOX * P8_D + ((c ^ (key & 7)) << 4));
+                    unsigned w[4] = {four.x, four.y, four.z, four.w};
+                    unsigned h[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (kv == 1) {
+                            if (!there) w[i] = 0u;
+                            const unsigned bad = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;         // bytes that are no number
+                            if (bad) {
+                                nan = true;
+                                w[i] &= ~((bad >> 7) * 0xffu);
+                            }
+                        }
+                        h[2 * i] = kv8_half2((unsigned short)w[i]);
+                        h[2 * i + 1] = kv8_half2((unsigned short)(w[i] >> 16));
+                    }
+                    unsigned char* line = dst + (c >> 2) * P8_HALF;
+                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + 1) ^ (key & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                }
+                if (kv == 1) {
+                    const unsigned any = __ballot_sync(0xffffffffu, nan);
+                    if (lane == 0) no_number[j % P8_SCALE_SLOTS][warp - 8] = any;
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    p8_arrive(kv == 0 ? &k_full : &v_full);
+                    if (kv == 1) p8_arrive(&raw_free[j & 1]);
+                }
+            }
+        }
+    } else {
+        // ---- softmax ----
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + mine * 128, to = tmem + lanes + 256 + mine * 128;
+        const int index = mine * P8_ROWS + row;
+        const bool live = index < rows;
+        const int pos = live ? pos0 + tok0 + index / G : -1;     // -1: a row that does not exist sees nothing
+        const int first = p.window > 0 ? pos - p.window + 1 : 0;
+        // positions of the tile's first and last row: what no key tile has to be masked for
+        const int pos_first = pos0 + tok0 + mine * P8_ROWS / G, pos_last = pos0 + tok0 + (min(rows, (mine + 1) * P8_ROWS) - 1) / G;
+        float m = -INFINITY, mu = -INFINITY, l = 0.f;
+        const int count = n[mine];
+        uint32_t a[32], b[32], pk[16];
+        for (int j = 0; j < count; ++j) {
+            const int j0 = (t_begin + j) * P8_KEYS, slot = j % P8_SCALE_SLOTS;
+            const bool mask = j0 + P8_KEYS - 1 > pos_first || (p.window > 0 && j0 < pos_last - p.window + 1) || rows < (mine + 1) * P8_ROWS;
+            const Tile8 tile{scales[slot], f, first - j0, pos - j0};
+            mbar_wait(&s_full[mine], j & 1, p.error_flag);       // P V of the key tile before is done as well: it was issued before
+            fa_fence_after();
+            float t_top = -INFINITY, u_top = -INFINITY;
+            auto top = [&](const uint32_t (&x)[32], int col) {
+                if (mask) p8_top<true>(x, col, tile, t_top, u_top); else p8_top<false>(x, col, tile, t_top, u_top);
+            };
+            FA_TMEM_LD32(ts, a, 0);
+            fa_tmem_wait_ld();
+            FA_TMEM_LD32(ts + 32, b, 0);
+            top(a, 0);
+            fa_tmem_wait_ld();
+            FA_TMEM_LD32(ts + 64, a, 0);
+            top(b, 32);
+            fa_tmem_wait_ld();
+            FA_TMEM_LD32(ts + 96, b, 0);
+            top(a, 64);
+            fa_tmem_wait_ld();
+            FA_TMEM_LD32(ts, a, 0);                              // the first columns again
+            top(b, 96);
+            if (t_top > m + 8.f) {
+                const float to_m = ceilf(t_top);
+                l *= m == -INFINITY ? 0.f : fa_ex2(m - to_m);
+                m = to_m;
+            }
+            float alpha = 1.f;
+            const bool raise = u_top > mu + 8.f;
+            if (raise) {
+                const float to_mu = ceilf(u_top);
+                alpha = fa_ex2(mu - to_mu);                      // 0 the first time
+                mu = to_mu;
+            }
+            fa_tmem_wait_ld();
+            if (j > 0 && __any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int c = 0; c < P8_D; c += 32) {
+                    FA_TMEM_LD32(to + c, b, 0);
+                    fa_tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) b[i] = __float_as_uint(__uint_as_float(b[i]) * alpha);
+                    FA_TMEM_ST32(to + c, b, 0);
+                }
+            }
+            const float m_now = m == -INFINITY ? 0.f : m, mu_now = mu == -INFINITY ? 0.f : mu;
+            auto factors = [&](const uint32_t (&x)[32], int col) {
+                if (mask) p8_factors<true>(x, col, tile, m_now, mu_now, pk, l); else p8_factors<false>(x, col, tile, m_now, mu_now, pk, l);
+            };
+            // factors over the first 64 columns of S, always over columns that were read before
+            FA_TMEM_LD32(ts + 32, b, 0);
+            factors(a, 0);
+            fa_tmem_wait_ld();
+            FA_TMEM_LD32(ts + 64, a, 0);
+            FA_TMEM_ST16(ts, pk);
+            factors(b, 32);
+            fa_tmem_wait_ld();
+            FA_TMEM_LD32(ts + 96, b, 0);
+            FA_TMEM_ST16(ts + 16, pk);
+            factors(a, 64);
+            fa_tmem_wait_ld();
+            FA_TMEM_ST16(ts + 32, pk);
+            factors(b, 96);
+            FA_TMEM_ST16(ts + 48, pk);
+            fa_tmem_wait_st();
+            fa_fence_before();
+            __syncwarp();
+            if (lane == 0) p8_arrive(&p_full[mine]);
+            // values that are no number: looked at once the tile's values are unpacked, which the next wait stands behind
+            if (j > 0) {
+                const int before = (j - 1) % P8_SCALE_SLOTS, k0 = j0 - P8_KEYS;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const unsigned bad = no_number[before][w];
+                    if (bad != 0u)
+                        for (int i = 0; i < 32; ++i)
+                            if ((bad >> i & 1u) && k0 + w * 32 + i >= first && k0 + w * 32 + i <= pos) l = __int_as_float(0x7fffffff);
+                }
+            }
+        }
+        if (count > 0) mbar_wait(&o_done[mine], (count - 1) & 1, p.error_flag);
+        fa_fence_after();
+        if (count > 0) {
+            const int before = (count - 1) % P8_SCALE_SLOTS, k0 = (t_begin + count - 1) * P8_KEYS;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const unsigned bad = no_number[before][w];
+                if (bad != 0u)
+                    for (int i = 0; i < 32; ++i)
+                        if ((bad >> i & 1u) && k0 + w * 32 + i >= first && k0 + w * 32 + i <= pos) l = __int_as_float(0x7fffffff);
+            }
+        }
+        const float inv = l == 0.f ? 0.f : exp2f(mu - m) / l;    // no keys: zeros
+        bf16* out = p.out + (size_t)(q_begin + tok0 + (live ? index / G : 0)) * p.out_stride + (size_t)(kvh * G + index % G) * P8_D;
+        float* sums = p.partials + (((size_t)item.w * p.nkv + kvh) * (2 * P8_ROWS) + index) * P8_PART;
+#pragma unroll
+        for (int c = 0; c < P8_D; c += 32) {
+            if (count > 0) {
+                FA_TMEM_LD32(to + c, a, 0);
+                fa_tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) a[i] = 0u;
+            }
+            if (!live) continue;
+            if (parts == 1) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    uint4 v;
+                    v.x = fa_pack(__uint_as_float(a[i]) * inv, __uint_as_float(a[i + 1]) * inv);
+                    v.y = fa_pack(__uint_as_float(a[i + 2]) * inv, __uint_as_float(a[i + 3]) * inv);
+                    v.z = fa_pack(__uint_as_float(a[i + 4]) * inv, __uint_as_float(a[i + 5]) * inv);
+                    v.w = fa_pack(__uint_as_float(a[i + 6]) * inv, __uint_as_float(a[i + 7]) * inv);
+                    *reinterpret_cast<uint4*>(out + c + i) = v;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(sums + c + i) = make_uint4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+            }
+        }
+        if (live && parts > 1) *reinterpret_cast<float4*>(sums + P8_D) = make_float4(m, mu, l, 0.f);
+    }
+    fa_fence_before();
+    __syncthreads();
+    if (warp == 13) {
+        fa_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Weight of a part's sum under a common maximum. One without a finite score has -inf: it is 0, or no number.
+__device__ __forceinline__ float p8_weight(float m, float common) { return m == -INFINITY ? 1.f : fa_ex2(m - common); }
+
+// A row of a row tile whose keys came in parts, a warp each: the parts' sums in order. `shared` [n][4]: request, first token, parts, first place.
+__global__ void __launch_bounds__(256) prompt_kv8_merge_kernel(const Prompt8Params p, const int* shared) {
+    pdl_trigger();
+    pdl_wait();
+    const int4 of = reinterpret_cast<const int4*>(shared)[blockIdx.y];
+    const int kvh = blockIdx.z, index = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int G = p.nq / p.nkv, q_begin = p.q_start[of.x], ntok = min(p.q_start[of.x + 1] - q_begin - of.y, p.tokens);
+    if (index >= ntok * G) return;
+    auto sums = [&](int part) { return p.partials + (((size_t)(of.w + part) * p.nkv + kvh) * (2 * P8_ROWS) + index) * P8_PART; };
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, mu = -INFINITY, l = 0.f;
+    for (int p0 = 0; p0 < of.z; p0 += 4) {                       // four parts on their way together
+        float4 v[4], s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            s[i] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+            if (p0 + i < of.z) {
+                v[i] = __ldcg(reinterpret_cast<const float4*>(sums(p0 + i)) + lane);
+                s[i] = __ldcg(reinterpret_cast<const float4*>(sums(p0 + i) + P8_D));
+            }
+        }
+        const float m_new = fmaxf(fmaxf(fmaxf(s[0].x, s[1].x), fmaxf(s[2].x, s[3].x)), m);
+        const float mu_new = fmaxf(fmaxf(fmaxf(s[0].y, s[1].y), fmaxf(s[2].y, s[3].y)), mu);
+        l *= p8_weight(m, m_new);
+        const float old = p8_weight(mu, mu_new);
+        o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            l = fmaf(s[i].z, p8_weight(s[i].x, m_new), l);
+            const float w = p8_weight(s[i].y, mu_new);
+            o.x = fmaf(v[i].x, w, o.x); o.y = fmaf(v[i].y, w, o.y); o.z = fmaf(v[i].z, w, o.z); o.w = fmaf(v[i].w, w, o.w);
+        }
+        m = m_new;
+        mu = mu_new;
+    }
+    const float inv = l == 0.f ? 0.f : exp2f(mu - m) / l;
+    bf16* out = p.out + (size_t)(q_begin + of.y + index / G) * p.out_stride + (size_t)(kvh * G + index % G) * P8_D + lane * 4;
+    *reinterpret_cast<uint2*>(out) = make_uint2(fa_pack(o.x * inv, o.y * inv), fa_pack(o.z * inv, o.w * inv));
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------------
+LLMP_API int llmp_kv8_prompt_supports(int nq, int nkv, int d, int page_size) {
+    return d == P8_D && nkv > 0 && nq % nkv == 0 && nq / nkv <= P8_ROWS && page_size >= 8 && (page_size & (page_size - 1)) == 0;
+}
+// Query tokens of an item, and floats of a place for its sums (all key/value heads).
+LLMP_API int llmp_kv8_prompt_tokens(int nq, int nkv) { return 2 * P8_ROWS / (nq / nkv); }
+LLMP_API long llmp_kv8_prompt_place_floats(int nkv) { return (long)nkv * 2 * P8_ROWS * P8_PART; }
+
+// items: [num_items][4] as in Prompt8Params; shared: [num_shared][4] as in prompt_kv8_merge_kernel; partials: the items' places.
+LLMP_API int llmp_kv8_prompt(const void* q, long q_stride, void* out, long out_stride, const void* pages, int num_pages, const int* block_tables,
+                             int table_stride, const int* q_start, const int* ctx_len, const int* items, int num_items, const int* shared,
+                             int num_shared, float* partials, int nq, int nkv, int page_size, int window, float scale, int* error_flag,
+                             cudaStream_t stream) {
+    if (num_items <= 0) return 0;
+    LLMP_REQUIRE(llmp_kv8_prompt_supports(nq, nkv, P8_D, page_size), "kv8 prompt attention: %d and %d heads, pages of %d tokens are not for this kernel", nq, nkv, page_size);
+    LLMP_REQUIRE((q_stride % 8) == 0 && (out_stride % 8) == 0 && ((size_t)q % 16) == 0 && ((size_t)out % 16) == 0 && ((size_t)pages % 16) == 0 &&
+                 ((size_t)items % 16) == 0 && ((size_t)shared % 16) == 0, "kv8 prompt attention: rows and lists must be 16-byte aligned");
+    LLMP_REQUIRE(error_flag != nullptr && num_pages > 0 && table_stride > 0, "kv8 prompt attention: an error flag, pages and tables are needed");
+    LLMP_REQUIRE(num_shared == 0 || (partials != nullptr && shared != nullptr), "kv8 prompt attention: shared items need places for their sums");
+    LLMP_REQUIRE((long)num_items * nkv < (1L << 31) && num_shared <= 65535 && nkv <= 65535, "kv8 prompt attention: too many items");
+    Prompt8Params p;
+    p.q = (const bf16*)q; p.out = (bf16*)out; p.pages = (const unsigned char*)pages; p.block_tables = block_tables; p.q_start = q_start;
+    p.ctx_len = ctx_len; p.items = items; p.partials = partials; p.q_stride = q_stride; p.out_stride = out_stride;
+    p.page_bytes = kv8_page_bytes(nkv, page_size, P8_D); p.table_stride = table_stride; p.num_pages = num_pages; p.nq = nq; p.nkv = nkv;
+    p.page_size = page_size; p.page_shift = 31 - __builtin_clz((unsigned)page_size); p.window = window; p.tokens = llmp_kv8_prompt_tokens(nq, nkv);
+    p.scale = scale; p.error_flag = error_flag;
+    const int box_tokens = page_size < 32 ? page_size : 32;
+    EncodeTiledFn encode = llmp_tensor_map_encoder();
+    LLMP_REQUIRE(encode != nullptr, "kv8 prompt attention: the driver does not provide cuTensorMapEncodeTiled");
+    CUtensorMap map;
+    const cuuint64_t row = P8_D, plane = row * page_size;
+    const cuuint64_t dims[5] = {P8_D, (cuuint64_t)page_size, (cuuint64_t)nkv, 2, (cuuint64_t)num_pages};
+    const cuuint64_t strides[4] = {row, plane, plane * nkv, (cuuint64_t)p.page_bytes};
+    const cuuint32_t box[5] = {P8_D, (cuuint32_t)box_tokens, 1, 2, 1};
+    const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+    const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    LLMP_REQUIRE(rc == CUDA_SUCCESS, "kv8 prompt attention: cuTensorMapEncodeTiled failed with code %d", (int)rc);
+    const size_t smem = 8 * (size_t)P8_HALF + 2 * (size_t)P8_RAW_STAGE + 1024;
+    const auto kernel = box_tokens == 8 ? prompt_kv8_kernel<8> : box_tokens == 16 ? prompt_kv8_kernel<16> : prompt_kv8_kernel<32>;
+    if (box_tokens == 8) LLMP_ALLOW_SMEM(prompt_kv8_kernel<8>, smem);
+    else if (box_tokens == 16) LLMP_ALLOW_SMEM(prompt_kv8_kernel<16>, smem);
+    else LLMP_ALLOW_SMEM(prompt_kv8_kernel<32>, smem);
+    llmp_launch_dependent(kernel, dim3((unsigned)num_items * nkv), dim3(P8_THREADS), smem, stream, map, p);
+    if (num_shared > 0) llmp_launch_dependent(prompt_kv8_merge_kernel, dim3(2 * P8_ROWS / 8, num_shared, nkv), dim3(256), 0, stream, p, shared);
+    return llmp_check_launch("kv8_prompt");
+}

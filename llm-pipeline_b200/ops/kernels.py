@@ -126,6 +126,7 @@ _SIGNATURES = {
     "llmp_kv8_gather": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P],
     "llmp_kv8_decode": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
     "llmp_kv8_stream": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P, _P],
+    "llmp_kv8_prompt": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P],
     "llmp_copy_pages": [_P, _I, _L, _P, _P, _I, _P],
 }
 _bound = {}
@@ -2453,6 +2454,42 @@ def kv8_decode_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
     _call("llmp_kv8_decode", at, q_stride, out.data_ptr(), width, dtype, pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
           block_tables.shape[1], ctx_len.data_ptr(), R, max_ctx, num_heads, num_kv_heads, head_dim, page_size, window, scale, scratch.data_ptr(),
           scratch.numel(), _stream())
+    return out
+
+
+@functools.lru_cache(maxsize=None)
+def kv8_prompt_supports(dtype: torch.dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
+    """Whether prompt portions over 8-bit pages of these sizes have a kernel that reads them as they are."""
+    return dtype == torch.bfloat16 and bool(library().llmp_kv8_prompt_supports(num_heads, num_kv_heads, head_dim, page_size))
+
+
+@functools.lru_cache(maxsize=None)
+def kv8_prompt_sizes(num_heads: int, num_kv_heads: int) -> Tuple[int, int]:
+    """Query tokens of an item of that kernel's list, and floats of a place for the sums of an item whose tile is shared."""
+    fn = library().llmp_kv8_prompt_place_floats
+    fn.argtypes, fn.restype = [_I], _L
+    return int(library().llmp_kv8_prompt_tokens(num_heads, num_kv_heads)), int(fn(num_kv_heads))
+
+
+def kv8_prompt_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, pages: torch.Tensor, block_tables: torch.Tensor, q_start: torch.Tensor,
+                         ctx_len: torch.Tensor, items: torch.Tensor, shared: torch.Tensor, places: int, num_heads: int, num_kv_heads: int,
+                         page_size: int, window: int, scale: float) -> torch.Tensor:
+    """Causal attention of a step's query rows (head size 128) over 8-bit pages. ``items`` int32 [n, 4]: request, first token, number of a
+    part of the tile's keys | parts << 16, place of the part's sums; ``shared`` int32 [m, 4]: request, first token, parts, first place of
+    every tile that comes in parts (``ops.kv8.PromptPlan`` makes both)."""
+    for name, t in (("block_tables", block_tables), ("q_start", q_start), ("ctx_len", ctx_len), ("items", items), ("shared", shared)):
+        _i32(t, name)
+    if not (items.dim() == shared.dim() == 2 and items.shape[1] == shared.shape[1] == 4):
+        raise KernelError("the lists of a prompt's items must be [n, 4]")
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.shape[1] != num_heads * 128:
+        raise KernelError("prompt attention over 8-bit pages takes bfloat16 queries and gives contiguous bfloat16 [tokens, heads * 128]")
+    _kv8_pages(pages, num_kv_heads, 128, page_size)
+    _on_current_device(q, out, pages, block_tables, q_start, ctx_len, items, shared)
+    partials = torch.empty(places * kv8_prompt_sizes(num_heads, num_kv_heads)[1], dtype=torch.float32, device=q.device) if places else None
+    _call("llmp_kv8_prompt", q.data_ptr(), q_stride, out.data_ptr(), out.stride(0), pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
+          block_tables.shape[1], q_start.data_ptr(), ctx_len.data_ptr(), items.data_ptr(), items.shape[0], shared.data_ptr() if places else None,
+          shared.shape[0], None if partials is None else partials.data_ptr(), num_heads, num_kv_heads, page_size, window, scale,
+          error_flag().data_ptr(), _stream())
     return out
 
 

@@ -1,27 +1,55 @@
 """Attention of prompt portions over pages of 8-bit keys and values (``cache.spec.KV8PagesSpec``).
 
-A page's values are exact in bfloat16 and float32 (the scales are powers of two), and the row tiles of a portion read the
-same pages many times. So the pages that a step's portions see are unpacked once per layer into a workspace of the
-query's type, laid out as ordinary pages, and the attention kernels of ordinary pages run over it
-(``kernels.paged_attention``): the result is exactly what they give for a cache that holds these values. Unpacking moves
-three bytes a value; 2,048 new tokens of a group of four heads compute 16,384 products with it."""
+bfloat16 queries of head size 128 have a kernel that reads the pages as they are (``kernels.kv8_prompt_attention``). For other
+sizes and for float32 the pages that a step's portions see are unpacked into a workspace of the query's type, laid out as ordinary
+pages, and the attention kernels of ordinary pages run over it (``kernels.paged_attention``): a page's values are exact in
+either type (the scales are powers of two), so the result is exactly what they give for a cache that holds these values."""
 
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, Sequence, Tuple
 
 import torch
 
 from . import kernels
 
-WORKSPACE_BYTES = 1 << 30            # requests whose unpacked pages pass this together take turns in the workspace
+WORKSPACE_BYTES = 1 << 30            # unpacked pages, and sums of items: requests (or parts of tiles) that pass this together take turns (or are not cut)
+KEY_TILE = 128                       # keys of a tile of the kernel that reads 8-bit pages
+# Key tiles of a part at least where a tile's keys are shared among items, which costs a launch and the sums' way through memory.
+PART_TILES = 4
+
+
+def plan_items(starts: Sequence[int], q_lens: Sequence[int], first_request: int, tokens: int, num_kv_heads: int, window: int, sms: int,
+               most_places: int) -> Tuple[List[List[int]], List[List[int]], int]:
+    """(items, shared, places) for ``kernels.kv8_prompt_attention``: every ``tokens`` new tokens of a request are a tile, whose keys come
+    in parts where that evens out the work of ``sms`` SMs that run one item and key/value head at a time (few new tokens over many
+    keys). The items that see most keys come first."""
+    tiles = []
+    for r in range(first_request, len(q_lens)):
+        for t in range(0, q_lens[r], tokens):
+            last = starts[r] + min(t + tokens, q_lens[r]) - 1
+            low = max(starts[r] + t - window + 1, 0) if window else 0
+            tiles.append((last // KEY_TILE + 1 - low // KEY_TILE, r, t))
+    share = max(PART_TILES, -(-sum(n for n, _r, _t in tiles) * num_kv_heads // sms))
+    parts = [-(-n // share) if n > 1.25 * share else 1 for n, _r, _t in tiles]
+    if sum(k for k in parts if k > 1) > most_places:
+        parts = [1] * len(tiles)
+    items, shared, places = [], [], 0
+    for i in sorted(range(len(tiles)), key=lambda i: (-tiles[i][0] / parts[i], tiles[i][1:])):
+        _n, r, t = tiles[i]
+        for k in range(parts[i]):
+            items.append([r, t, k | parts[i] << 16, places + k if parts[i] > 1 else 0])
+        if parts[i] > 1:
+            shared.append([r, t, parts[i], places])
+            places += parts[i]
+    return items, shared, places
 
 
 class PromptPlan:
-    """What a step's prompt attention needs besides its tensors: which pages are unpacked to where, and the work list of the
-    attention kernel. One plan serves every layer of a step with the same heads, head size, page size and window.
-    ``starts`` and ``q_lens``: cached tokens and new tokens of every request, as host numbers; the requests before ``first_request``
-    are left out (their rows of the output are not written). Its lists are made on the stream that is current when it is first used."""
+    """What a step's prompt attention needs besides its tensors. One plan serves every layer of a step with the same heads, head size,
+    page size and window. ``starts`` and ``q_lens``: cached tokens and new tokens of every request, as host numbers; the requests
+    before ``first_request`` are left out (their rows of the output are not written). Its lists are made on the stream that is
+    current when it is first used."""
 
     def __init__(self, starts: Sequence[int], q_lens: Sequence[int], num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                  window: int, dtype: torch.dtype, device: torch.device, first_request: int = 0):
@@ -33,9 +61,12 @@ class PromptPlan:
         self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
         self.page_size, self.window, self.dtype, self.device = page_size, window, dtype, torch.device(device)
         self.first_request = first_request
+        self.rows = sum(self.q_lens)
+        self.longest = max((s + n for s, n in zip(self.starts, self.q_lens)), default=0)
         self.page_bytes = 2 * num_kv_heads * page_size * head_dim * dtype.itemsize
         self.groups = self._groups()
         self._lists: Dict[int, list] = {}            # by the width of the block tables
+        self._items = None
 
     def pages_of(self, r: int) -> Tuple[int, int]:
         """The pages (first, end) of request r that its new tokens see."""
@@ -43,7 +74,7 @@ class PromptPlan:
         return first // self.page_size, -(-(self.starts[r] + self.q_lens[r]) // self.page_size)
 
     def _groups(self) -> List[List[int]]:
-        """The requests with new tokens, in runs whose pages fit the workspace together (a request alone may pass it)."""
+        """The requests with new tokens, in runs whose unpacked pages fit the workspace together (a request alone may pass it)."""
         groups: List[List[int]] = []
         room = 0
         for r in range(self.first_request, len(self.q_lens)):
@@ -58,6 +89,25 @@ class PromptPlan:
             room -= size
         return groups
 
+    def _on_device(self, lists: Sequence[torch.Tensor]) -> List[torch.Tensor]:
+        """The int32 lists through one pinned copy, each from a multiple of 16 bytes on."""
+        padded = [torch.nn.functional.pad(t.flatten(), (0, -t.numel() % 4)) for t in lists]
+        dev, at, out = torch.cat(padded).pin_memory().to(self.device, non_blocking=True), 0, []
+        for t, room in zip(lists, padded):
+            out.append(dev[at:at + t.numel()].view(t.shape))
+            at += room.numel()
+        return out
+
+    def items(self):
+        """(items, shared, places) on the device for the kernel that reads 8-bit pages."""
+        if self._items is None:
+            tokens, floats = kernels.kv8_prompt_sizes(self.num_heads, self.num_kv_heads)
+            items, shared, places = plan_items(self.starts, self.q_lens, self.first_request, tokens, self.num_kv_heads, self.window,
+                                               kernels.sm_count(), WORKSPACE_BYTES // (4 * floats))
+            lists = [torch.tensor(rows, dtype=torch.int32).reshape(len(rows), 4) for rows in (items, shared)]
+            self._items = (*self._on_device(lists), places)
+        return self._items
+
     def lists(self, table_width: int) -> list:
         """Per group: (entries of the block tables to unpack, block tables of the workspace, tile_req, tile_tok0, tile_seg, tile_slot,
         places, tokens per tile), on the device."""
@@ -71,23 +121,18 @@ class PromptPlan:
         tokens, segments = kernels.tokens_per_attention_tile(*sizes), kernels.attention_max_segments(*sizes)
         for group in self.groups:
             width = max(self.pages_of(r)[1] for r in group)
-            kernels._need(width <= table_width, f"a request sees {width} pages, its block table has {table_width}")
             index: List[int] = []
             tables = torch.full((R, width), -1, dtype=torch.int32)
             for r in group:
                 first, end = self.pages_of(r)
                 tables[r, first:end] = torch.arange(len(index), len(index) + end - first, dtype=torch.int32)
                 index.extend(range(r * table_width + first, r * table_width + end))
-            alone = [n if r in set(group) else 0 for r, n in enumerate(self.q_lens)]
+            mine = set(group)
+            alone = [n if r in mine else 0 for r, n in enumerate(self.q_lens)]
             req, tok0, seg, slot, places = AttentionPolicy.plan_items(self.starts, alone, tokens, 0, segments, self.num_kv_heads,
                                                                       kernels.sm_count())
-            rows = [req, tok0] + ([seg, slot] if places else [])
-            flat = torch.cat([torch.tensor(index, dtype=torch.int32), tables.flatten(), torch.tensor(rows, dtype=torch.int32).flatten()])
-            dev = flat.pin_memory().to(self.device, non_blocking=True)
-            at = len(index)
-            items = dev[at + R * width:].view(len(rows), len(req))
-            made.append((dev[:at], dev[at:at + R * width].view(R, width), items[0], items[1], items[2] if places else None,
-                         items[3] if places else None, places, tokens))
+            lists = [torch.tensor(index, dtype=torch.int32), tables] + [torch.tensor(x, dtype=torch.int32) for x in (req, tok0, seg, slot)]
+            made.append((*self._on_device(lists)[:4 if not places else 6], *(() if places else (None, None)), places, tokens))
         self._lists[table_width] = made
         return made
 
@@ -95,14 +140,27 @@ class PromptPlan:
 def prompt_attention(plan: PromptPlan, q: torch.Tensor, q_stride: int, out: torch.Tensor, pages: torch.Tensor, block_tables: torch.Tensor,
                      q_start: torch.Tensor, ctx_len: torch.Tensor, scale: float) -> torch.Tensor:
     """Causal attention of the step's query rows over 8-bit pages, any portion sizes: as ``kernels.paged_attention`` over pages
-    that hold the same values in q's type. ``q_start`` and ``ctx_len`` are the plan's lengths on the device."""
+    that hold the same values in q's type. ``q_start`` and ``ctx_len`` are the plan's lengths on the device. Every page that the new
+    tokens see has to be there."""
     nq, nkv, d, ps = plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.page_size
     kernels._kv8_pages(pages, nkv, d, ps)
-    kernels._need(q.dtype == plan.dtype, f"the plan is for queries in {plan.dtype}")
-    kernels._need(block_tables.dim() == 2 and block_tables.shape[0] == len(plan.q_lens) == ctx_len.numel() and
-                  q_start.numel() == len(plan.q_lens) + 1, "block tables, q_start and ctx_len must be those of the plan's requests")
-    kernels._need(q.dim() == 2 and q.stride(1) == 1 and q.stride(0) == q_stride or q.shape[0] <= 1, "query rows must lie q_stride apart")
-    kernels._need(q.shape[0] >= sum(plan.q_lens) and out.shape[0] >= sum(plan.q_lens), "the plan has more rows than the queries or the output")
+    if q.dtype != plan.dtype:
+        raise kernels.KernelError(f"the plan is for queries in {plan.dtype}")
+    R = len(plan.q_lens)
+    if not (block_tables.dim() == 2 and block_tables.shape[0] == R == ctx_len.numel() and q_start.numel() == R + 1):
+        raise kernels.KernelError("block tables, q_start and ctx_len must be those of the plan's requests")
+    if not (q.dim() == 2 and q.shape[1] >= nq * d and (q.shape[0] <= 1 or (q.stride(1) == 1 and q.stride(0) == q_stride))):
+        raise kernels.KernelError("query rows must hold the plan's heads and lie q_stride apart")
+    if q.shape[0] < plan.rows or out.shape[0] < plan.rows:
+        raise kernels.KernelError("the plan has more rows than the queries or the output")
+    if block_tables.shape[1] * ps < plan.longest:
+        raise kernels.KernelError(f"a request sees {plan.longest} tokens, its block table has room for {block_tables.shape[1] * ps}")
+    if not plan.groups:
+        return out
+    if kernels.kv8_prompt_supports(q.dtype, nq, nkv, d, ps) and (q.data_ptr() | 2 * q_stride | out.data_ptr()) % 16 == 0:
+        items, shared, places = plan.items()
+        return kernels.kv8_prompt_attention(q, q_stride, out, pages, block_tables, q_start, ctx_len, items, shared, places, nq, nkv, ps,
+                                            plan.window, scale)
     kernels._on_current_device(q, out, pages, block_tables, q_start, ctx_len)
     for index, tables, req, tok0, seg, slot, places, tokens in plan.lists(block_tables.shape[1]):
         held = torch.empty((index.numel(), 2, nkv, ps, d), dtype=q.dtype, device=q.device)

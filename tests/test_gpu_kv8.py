@@ -357,6 +357,86 @@ def test_prompt_portions(dtype, nq, nkv, d, ps, portions, window):
     assert bool((out[at:] == 9).all())                                           # rows behind the last request's
 
 
+@pytest.mark.parametrize("nq,nkv,d,ps,starts,lens", [(32, 8, 128, 16, [5000], [40]), (32, 8, 128, 8, [3001, 0], [3, 200]), (8, 8, 128, 32, [700, 2000], [1, 300]),
+                                                     (40, 2, 128, 16, [4000], [17]), (9, 1, 128, 64, [6000], [5]), (32, 8, 128, 128, [0], [1111])])
+@pytest.mark.parametrize("window", [0, 2000])
+def test_prompt_portions_on_the_tensor_cores(nq, nkv, d, ps, starts, lens, window):
+    """Few new tokens over many keys (their keys come in parts), odd groups, pages of every size, values of very different scales."""
+    host, tables, ctx, q, out = prompt((nq, nkv, d, ps), starts, lens, window, torch.bfloat16, 61)
+    check_prompt(host, tables, ctx, q, out, starts, lens, nq, nkv, d, window)
+
+
+def check_prompt(host, tables, ctx, q, out, starts, lens, nq, nkv, d, window, skip=()):
+    at = 0
+    for r, n in enumerate(lens):
+        k, v, there = host.request(tables[r], ctx[r])
+        for i in sorted({0, 1, n // 3, n // 2, n - 2, n - 1} & set(range(n)) - set(skip)):
+            row, pos = q[at + i:at + i + 1, :nq * d].view(1, nq, d), starts[r] + i
+            seen = slice(max(0, pos - window + 1) if window else 0, pos + 1)
+            kk, vv, tt = k[seen], v[seen], there[seen]
+            want, size, top = plain.attend(row, kk, vv, [len(kk) - 1], tt, d ** -0.5, 0)
+            allowed = bound(want, size, top, torch.bfloat16, d) + plain.smallest(row[0], kk, vv, host.value_scales(tables[r], ctx[r])[seen], len(kk) - 1, tt,
+                                                                                d ** -0.5, 0)       # as for single tokens
+            far = (out[at + i].double().cpu().view(1, nq, d) - want).abs()
+            assert bool((far <= allowed).all()), f"request {r} row {i}: {float((far / allowed).max())}"
+        at += n
+    assert bool((out[at:] == 9).all())
+
+
+def test_prompt_portions_over_blocks_of_very_different_scales():
+    """Value blocks from 2^-60 to 2^60 and blocks of zeros; keys of very different sizes; queries of zeros and of 1e-30."""
+    from llm_pipeline_b200.ops import kv8
+
+    nq, nkv, d, ps, starts, lens = 32, 8, 128, 16, [333, 0], [100, 150]
+    gen = torch.Generator().manual_seed(3)
+    ctx = [433, 150]
+    P = 40
+    host = filled(P, nkv, ps, d, 71)
+    host.e[:, 1] = torch.randint(67, 188, host.e[:, 1].shape, generator=gen).to(torch.uint8)
+    empty = torch.rand(host.e[:, 1].shape, generator=gen) < 0.3
+    host.e[:, 1][empty] = 0
+    host.q[:, 1][empty] = 0
+    host.e[::5, 0] = 0
+    host.q[::5, 0] = 0
+    tables = scattered(ctx, ps, P, 5)
+    q = torch.randn(250, nq * d, generator=gen)
+    q[3] = 0
+    q[100] *= 1e-30
+    q = q.bfloat16()
+    out = torch.full((250, nq * d), 9.0, dtype=torch.bfloat16, device=DEV)
+    plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, 0, torch.bfloat16, torch.device(DEV))
+    kv8.prompt_attention(plan, q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), torch.tensor([0, 100, 250], dtype=torch.int32, device=DEV),
+                         torch.tensor(ctx, dtype=torch.int32, device=DEV), d ** -0.5)
+    check_prompt(host, tables, ctx, q, out, starts, lens, nq, nkv, d, 0)
+
+
+@pytest.mark.parametrize("dim,ps", [(128, 16)])
+def test_what_a_row_cannot_see_does_not_matter_to_it(dim, ps):
+    """Keys and values that are no number, of tokens that come after a row or before its window, leave the row as it is; rows that see them
+    are no number; a query that is none is its own row's matter."""
+    nq, nkv, starts, lens, window = 8, 2, [200], [300], 150
+    host, tables, ctx, q, clean = prompt((nq, nkv, dim, ps), starts, lens, window, torch.bfloat16, 81)
+    from llm_pipeline_b200.ops import kv8
+
+    at = 320                                                                     # a token of the portion: rows 120 .. 269 see it
+    host.q[int(tables[0, at // ps]), 1, 0, at % ps, 7] = 127                     # a value of head 0
+    host.q[int(tables[0, at // ps]), 0, 1, at % ps, 9] = 255                     # a key of head 1
+    q[5, 3 * dim] = float("nan")
+    out = torch.full_like(clean, 9.0)
+    plan = kv8.PromptPlan(starts, lens, nq, nkv, dim, ps, window, torch.bfloat16, torch.device(DEV))
+    kv8.prompt_attention(plan, q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), torch.tensor([0, 300], dtype=torch.int32, device=DEV),
+                         torch.tensor(ctx, dtype=torch.int32, device=DEV), dim ** -0.5)
+    nan = out[:300].view(300, nq, dim).isnan()
+    sees = torch.zeros(300, dtype=torch.bool, device=DEV)
+    sees[120:270] = True
+    assert bool(nan[sees].all(-1).all()) or bool(nan[sees][:, 4:].all())
+    assert bool(nan[sees].any(-1).all())
+    assert not bool(nan[~sees].sum() - nan[5, 3].sum()) and bool(nan[5, 3].all())
+    rest = ~sees[:, None].expand(300, nq).clone()
+    rest[5, 3] = False
+    assert torch.equal(out[:300].view(300, nq, dim)[rest], clean[:300].view(300, nq, dim)[rest])
+
+
 def test_prompt_portions_in_turns_of_a_small_workspace(monkeypatch):
     from llm_pipeline_b200.ops import kv8
 
