@@ -2,24 +2,27 @@
 // queries, head size 128, as llmp_paged_attention over pages of bfloat16.
 //
 // A block takes 256 query rows of one request and one key/value head (a row is a token and a query head of the group, the head running
-// fastest) as two tiles of 128, and walks tiles of 128 keys. All products are in half precision, which holds every e4m3 value exactly:
-//   unpack       four warps turn a tile's bytes into half precision, laid out as operands; both row tiles use what is unpacked once
+// fastest) as two tiles of 128, and walks tiles of 128 keys. All products are in half precision, which holds every e4m3 value (and 2^-8 of it) exactly:
+//   unpack       six warps turn a tile's bytes into half precision, laid out as operands; both row tiles use what is unpacked once. By
+//                shifts and masks: the conversion instruction is as slow as the exponentials and shares their unit
 //   S = Q K^T    Q, K in shared memory (128-byte swizzle, K-major), S in tensor memory
-//   softmax      a thread has a row: it reads S from tensor memory twice, 32 columns at a time, and writes factors over S
+//   softmax      a thread has a row: it reads S from tensor memory twice (maxima; factors), 32 columns at a time in loops that stay
+//                short (unrolled whole, the instructions do not come fast enough: 112 us for 2,048 tokens), and writes factors over S
 //   O += P V     P read from tensor memory, V in shared memory MN-major, O in tensor memory
 // While one row tile is in its softmax the tensor cores work for the other. The two tiles' S and O fill the tensor memory (512 columns).
 //
 // With t = log2(e) scale q.k and a value's scale 2^v, weights are 2^t and the factor of a value's bytes is 2^(t + v). As in
-// attention_decode_kv8_stream.cu each has its own maximum, m and mu, raised to a whole number when it is passed by more than 8: factors
-// are held in half precision relative to 2^mu, the sum l of the weights in float32 relative to 2^m, and out = O / l * 2^(mu - m). A
-// block of eight keys has one scale, so a weight is its factor times 2^(mu - m - v), a power of two; only where that is beyond 2^100 are
-// the weights computed apart. Queries are brought to a largest magnitude in [1, 4) by a power of two per row.
+// attention_decode_kv8_stream.cu each has its own maximum, m and mu, raised to a whole number when it is passed by more than 12: factors
+// are held in half precision relative to 2^mu, the sum l of the weights in float32 relative to 2^m, and out = O / l * 2^(mu - m). The keys
+// of a page have one scale, so a weight is its factor times 2^(mu - m - v), a power of two; only where that is beyond 2^100 are the weights
+// computed apart. Queries are brought to a largest magnitude in
+// [1, 4) by a power of two per row, which takes the sign of the scale along.
 //
-// What cannot be seen does not matter: values behind the context and in missing pages are zeros as operands; a value that is no number is
-// one too, and the rows that see its key become no number by their l.
+// What cannot be seen does not matter: bytes behind the context and in missing pages are zeros as operands; those that are no number are
+// too, and the rows that see their key become no number by their l.
 //
-// Roles: warps 0-3 and 4-7 softmax of the two row tiles, 8-11 unpacking, 12 loads (TMA, a page and head in a box, keys and values
-// together), 13 issues the products. Few rows over many keys: an item of the list is a part of a row tile's keys and leaves its sums
+// Roles: warps 0-3 and 4-7 softmax of the two row tiles, 8-13 unpacking, 14 loads (TMA, a page and head in a box, keys and values
+// together), 15 issues the products. Few rows over many keys: an item of the list is a part of a row tile's keys and leaves its sums
 // in global memory, and prompt_kv8_merge_kernel adds them up. Every wait on an mbarrier is bounded: when one runs out the kernel records
 // 1 in *error_flag and goes on without waiting (its output is then wrong; the host reads the flag).
 #include "kv8.cuh"
@@ -29,10 +32,12 @@
 #define P8_D 128
 #define P8_ROWS 128                                  // of a row tile
 #define P8_KEYS 128
-#define P8_THREADS 448
+#define P8_THREADS 512
+#define P8_STAGES 2                                  // tiles of bytes on their way or being unpacked
+#define P8_UNPACK 6                                  // warps that unpack
 #define P8_HALF (P8_ROWS * 128)                      // bytes of 128 rows of 64 entries in half precision
 #define P8_RAW_STAGE (2 * P8_KEYS * P8_D)            // bytes of a tile's keys and values
-#define P8_SCALE_SLOTS 4                             // a tile's scales live until its softmax: at most four tiles are on their way
+#define P8_SLOTS 8                                   // places for a tile's scales, which live until its softmax is done
 #define P8_PART (P8_D + 4)                           // floats of a row's sums: O, m, mu, l
 
 struct Prompt8Params {
@@ -78,93 +83,111 @@ __device__ __forceinline__ unsigned p8_half2(float lo, float hi) {
 // 2^n for whole numbers -126 <= n <= 127 in a float, by its bits.
 __device__ __forceinline__ float p8_power(float n) { return __int_as_float((__float_as_int(n + 12582912.f) + 127) << 23); }
 
-// The keys of a tile that one row sees are first .. last (in the tile); the scales of its blocks of eight keys.
-struct Tile8 {
-    const float2* scales;                            // of the 16 blocks: the keys' scale times nothing yet, the exponent of the values'; missing: 0, -inf
-    float f;                                         // log2(e) * scale * the query row's own power of two
-    int first, last;
-};
+__device__ __forceinline__ float p8_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Pairs of floats in one instruction: x * c + add, and a + b.
+__device__ __forceinline__ float2 p8_fma2(float2 x, float2 c, float2 add) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, c, a, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\tmov.b64 a, {%6, %7};\n\t"
+        "fma.rn.f32x2 r, x, c, a;\n\tmov.b64 {%0, %1}, r;\n\t}\n" : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(c.x), "f"(c.y), "f"(add.x), "f"(add.y));
+    return r;
+}
+__device__ __forceinline__ float2 p8_add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}\n"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
 
-// The largest t and t + v among 32 scores, of the tile's columns from `col` on.
-template <bool MASK>
-__device__ __forceinline__ void p8_top(const uint32_t (&x)[32], int col, const Tile8& tile, float& t_top, float& u_top) {
+// Waits for this thread's tensor-memory loads. What they brought is named as changed by it: else the compiler may use the registers, which
+// it takes to be loaded where the load stands, before the wait.
+__device__ __forceinline__ void p8_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]) :: "memory");
+    asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+
+// The largest t and t + v of 32 scores (hidden ones are -inf). `scales`: of the 32 / BLOCK blocks they belong to, every BLOCK / 8th: the
+// keys' scale, the exponent of the values' (-inf: a page that is missing).
+template <int BLOCK> __device__ __forceinline__ void p8_top(const uint32_t (&x)[32], const float2* scales, float f, float& t_top, float& u_top) {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const float2 s = tile.scales[col / 8 + b];
-        float top = -INFINITY;
+    for (int b = 0; b < 32; b += BLOCK) {
+        const float2 s = scales[b / 8];
+        float top = fmaxf(__uint_as_float(x[b]), __uint_as_float(x[b + 1]));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int key = col + b * 8 + i;
-            const float v = __uint_as_float(x[b * 8 + i]);
-            if (!MASK || (key >= tile.first && key <= tile.last)) top = fmaxf(top, v);
-        }
-        const bool none = s.y == -INFINITY || (MASK && top == -INFINITY);
-        const float t = none ? -INFINITY : top * (s.x * tile.f);
+        for (int i = 2; i < BLOCK; i += 2) top = p8_max3(top, __uint_as_float(x[b + i]), __uint_as_float(x[b + i + 1]));
+        const float t = s.y == -INFINITY ? -INFINITY : top * fmaxf(s.x * f, 1e-38f);
         t_top = fmaxf(t_top, t);
         u_top = fmaxf(u_top, t + s.y);
     }
 }
 
-// The factors of 32 scores as pairs in half precision; adds their weights to l.
-template <bool MASK>
-__device__ __forceinline__ void p8_factors(const uint32_t (&x)[32], int col, const Tile8& tile, float m, float mu, uint32_t (&pk)[16], float& l) {
+// 32 scores -> 16 pairs of factors; returns the sum of their weights relative to 2^m.
+template <int BLOCK>
+__device__ __forceinline__ float p8_factors(const uint32_t (&x)[32], const float2* scales, float f, float m, float mu, uint32_t (&pk)[16]) {
+    float l = 0.f;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const float2 s = tile.scales[col / 8 + b];
-        const float c = s.x * tile.f, add = s.y - mu;
-        float p[8];
+    for (int b = 0; b < 32; b += BLOCK) {
+        const float2 s = scales[b / 8];
+        const float c = fmaxf(s.x * f, 1e-38f), add = s.y - mu;  // (not 0: a hidden score stays -inf)
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int key = col + b * 8 + i;
-            p[i] = fa_ex2(fmaf(__uint_as_float(x[b * 8 + i]), c, add));
-            if (MASK && (key < tile.first || key > tile.last)) p[i] = 0.f;
+        for (int i = 0; i < BLOCK; i += 2) {
+            const float2 u = p8_fma2(make_float2(__uint_as_float(x[b + i]), __uint_as_float(x[b + i + 1])), make_float2(c, c), make_float2(add, add));
+            const float2 v = make_float2(fa_ex2(u.x), fa_ex2(u.y));
+            sum = i == 0 ? v : p8_add2(sum, v);
+            pk[(b + i) / 2] = p8_half2(v.x, v.y);
         }
+        const float n = mu - m - s.y;                            // weight = factor * 2^n
+        if (__builtin_expect(n <= 100.f, 1)) {
+            l = fmaf(sum.x + sum.y, p8_power(fmaxf(n, -126.f)), l);
+        } else if (s.y > -INFINITY) {                            // factors too small for float32 although their weights are not
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pk[b * 4 + i] = p8_half2(p[2 * i], p[2 * i + 1]);
-        const float n = mu - m - s.y;                // weight = factor * 2^n
-        if (n <= 100.f) {
-            l = fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), p8_power(fmaxf(n, -126.f)), l);
-        } else if (s.y > -INFINITY) {                // factors too small for float32 although their weights are not
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int key = col + b * 8 + i;
-                if (!MASK || (key >= tile.first && key <= tile.last)) l += fa_ex2(fmaf(__uint_as_float(x[b * 8 + i]), c, -m));
-            }
+            for (int i = 0; i < BLOCK; ++i) l += fa_ex2(fmaf(__uint_as_float(x[b + i]), c, -m));
         }
     }
+    return l;
 }
 
 template <int BOX>
 __global__ void __launch_bounds__(P8_THREADS, 1)
 prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p) {
     extern __shared__ unsigned char p8_raw[];
-    __shared__ __align__(8) uint64_t raw_full[2], raw_free[2], k_full, k_free, v_full, v_free, s_full[2], p_full[2], o_done[2];
-    __shared__ __align__(16) float2 scales[P8_SCALE_SLOTS][16];
-    __shared__ unsigned no_number[P8_SCALE_SLOTS][4];            // keys of a tile whose values hold NaN
+    __shared__ __align__(8) uint64_t raw_full[P8_STAGES], raw_free[P8_STAGES], k_full, k_free, v_full[2], v_free[2], s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(16) float2 scales[P8_SLOTS][16];
+    __shared__ unsigned no_number[P8_SLOTS][4];            // keys of a tile whose values hold NaN
     __shared__ uint32_t tmem_slot;
     const uint32_t raw_addr = tc_smem_u32(p8_raw);
     unsigned char* Qs = p8_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);     // [2 tiles][2 halves][128 rows][128 bytes]
     unsigned char* Ks = Qs + 4 * P8_HALF;                        // [2 halves][128 keys][128 bytes]
     unsigned char* Vs = Ks + 2 * P8_HALF;
-    unsigned char* raw = Vs + 2 * P8_HALF;                       // [2 stages][box][keys, values][token][128 bytes]
+    unsigned char* raw = Vs + 4 * P8_HALF;                       // (two tiles of values before it) [P8_STAGES][box][keys, values][token][128 bytes]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (warp == 12 && lane == 0) {
-        for (int i = 0; i < 2; ++i) {
+    if (warp == 8 && lane == 0) {
+        for (int i = 0; i < P8_STAGES; ++i) {
             mbar_init(&raw_full[i], 2);                          // the boxes, and the scales
-            mbar_init(&raw_free[i], 4);
+            mbar_init(&raw_free[i], P8_UNPACK);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&v_full[i], P8_UNPACK);
+            mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
         }
-        mbar_init(&k_full, 4);
+        mbar_init(&k_full, P8_UNPACK);
         mbar_init(&k_free, 1);
-        mbar_init(&v_full, 4);
-        mbar_init(&v_free, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
     }
-    if (warp == 13) {
+    if (warp == 15) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
@@ -183,7 +206,8 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
     // keys of the whole row tile, and this part's tiles of them; a row tile of 128 rows sees none beyond its last row's position
     const int low = p.window > 0 ? max(pos0 + tok0 - p.window + 1, 0) : 0;
     const int tile0 = low / P8_KEYS, all_tiles = (pos0 + tok0 + ntok - 1) / P8_KEYS + 1 - tile0;
-    const int t_begin = tile0 + (int)((long)all_tiles * part / parts), t_end = tile0 + (int)((long)all_tiles * (part + 1) / parts);
+    const int each = all_tiles / parts, more = all_tiles - each * parts;         // the first `more` parts have one more
+    const int t_begin = tile0 + each * part + min(part, more), t_end = t_begin + each + (part < more);
     int n[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -214,15 +238,18 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         }
         int e = (int)(__float_as_uint(amax) >> 23);              // 2^(e - 127) <= amax < 2^(e - 126)
         e = e < 1 ? 1 : (e > 253 ? 253 : e);
-        const float down = kv8_power(127 - e);
-        f = p.scale * 1.4426950408889634f * kv8_power(e - 127);
+        const float down = p.scale < 0.f ? -kv8_power(127 - e) : kv8_power(127 - e);
+        f = fabsf(p.scale) * 1.4426950408889634f * kv8_power(e - 127);
         unsigned char* to = Qs + (size_t)mine * 2 * P8_HALF + row * 128;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
             const unsigned w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
             unsigned h[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = p8_half2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
+            for (int i = 0; i < 4; i += 2) {                     // entries 0, 2 and 1, 3 of four, as the keys are unpacked
+                h[i] = p8_half2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i + 1] << 16) * down);
+                h[i + 1] = p8_half2(__uint_as_float(w[i] & 0xffff0000u) * down, __uint_as_float(w[i + 1] & 0xffff0000u) * down);
+            }
             *reinterpret_cast<uint4*>(to + (c >> 3) * P8_HALF + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -232,8 +259,52 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
     fa_fence_after();
     const uint32_t tmem = tmem_slot;                             // S of the tiles in columns 0 and 128, O in 256 and 384
 
-    if (warp == 12) {
-        // ---- loads: lane b < 16 sees to block b of eight keys; page numbers two tiles ahead, scale bytes one ----
+    if (warp == 15) {
+        // ---- products ----
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = p8_idesc(P8_ROWS, P8_KEYS), idesc_o = p8_idesc(P8_ROWS, P8_D) | (1u << 16);      // V is MN-major
+            // (an operand further on in shared memory: its address in units of 16 bytes, in the descriptor's low bits)
+            const uint64_t q_desc = umma_desc(tc_smem_u32(Qs)), k_desc = umma_desc(tc_smem_u32(Ks)), v_desc = p8_desc_mn(tc_smem_u32(Vs));
+            const int last_t = n[1] > 0 ? 1 : 0;
+            // S of row tile t and key tile j; the first of the row tiles waits for the keys, the last frees them
+            auto scores = [&](int t, int j) {
+                if (t == 0 || j >= n[0]) mbar_wait(&k_full, j & 1, p.error_flag);
+                // S lies where the P of the key tile before is: products into other columns keep no order among themselves
+                if (j > 0) mbar_wait(&o_done[t], (j - 1) & 1, p.error_flag);
+                fa_fence_after();
+                const uint64_t q_at = q_desc + (uint32_t)t * (2 * P8_HALF >> 4);
+#pragma unroll
+                for (int k = 0; k < P8_D / 16; ++k) {
+                    const uint32_t off = ((uint32_t)(k >> 2) * P8_HALF + (uint32_t)(k & 3) * 32) >> 4;
+                    umma_f16(tmem + t * 128, q_at + off, k_desc + off, idesc_s, k != 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[t]);
+                if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&k_free);
+            };
+#pragma unroll 1
+            for (int j = -1; j < tiles; ++j) {
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t) {
+                    const int count = t == 0 ? n[0] : n[1];
+                    if (j >= count) continue;
+                    if (j < 0) {
+                        if (count > 0) scores(t, 0);
+                        continue;
+                    }
+                    mbar_wait(&p_full[t], j & 1, p.error_flag);
+                    if (t == 0 || j >= n[0]) mbar_wait(&v_full[j & 1], (j >> 1) & 1, p.error_flag);
+                    fa_fence_after();
+#pragma unroll
+                    for (int k = 0; k < P8_KEYS / 16; ++k)       // 16 keys a product: 8 columns of P, 2 KB of V
+                        fa_umma_a_tmem(tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc + (uint32_t)(((j & 1) * 2 * P8_HALF + k * 2048) >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
+                    umma_commit(&o_done[t]);
+                    if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&v_free[j & 1]);
+                    if (j + 1 < count) scores(t, j + 1);
+                }
+            }
+        }
+    } else if (warp == 14) {
+        // ---- loads: lane b < 16 sees to block b of eight keys; page numbers are asked for two tiles before their boxes, scale bytes one ----
         const bool boxes = lane < 16 && (lane * 8) % BOX == 0;
         const size_t body = (size_t)2 * p.nkv * p.page_size * P8_D;
         auto find = [&](int j) {
@@ -252,103 +323,69 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         int now = find(0), next = find(1);
         ask(now);
         for (int j = 0; j < tiles; ++j) {
-            const int after = find(j + 2), stage = j & 1;
-            if (j > 1) mbar_wait(&raw_free[stage], ((j >> 1) - 1) & 1, p.error_flag);
+            const int after = find(j + 2), stage = j % P8_STAGES;
+            if (j >= P8_STAGES) mbar_wait(&raw_free[stage], (j / P8_STAGES - 1) & 1, p.error_flag);
             if (lane == 0) mbar_expect_tx(&raw_full[stage], P8_RAW_STAGE);
             __syncwarp();
             if (boxes)                                           // out of range: the box arrives as zeros
                 p8_load_box(raw + stage * P8_RAW_STAGE + lane * 8 * 2 * P8_D, &map, ((t_begin + j) * P8_KEYS + lane * 8) & (p.page_size - 1), kvh,
                             now >= 0 ? now : p.num_pages, &raw_full[stage]);
-            if (lane < 16) scales[j % P8_SCALE_SLOTS][lane] = now >= 0 ? make_float2(kv8_scale(ek), (float)((int)ev - 127)) : make_float2(0.f, -INFINITY);
+            if (lane < 16)                                       // (a block of zeros may have any scale; the operands are 2^-8 of the bytes' values)
+                scales[j % P8_SLOTS][lane] = now >= 0 ? make_float2((ek == 0u ? 1.f : kv8_scale(ek)) * 256.f, (float)((int)ev - 119)) : make_float2(1.f, -INFINITY);
+            if (lane < 4) no_number[j % P8_SLOTS][lane] = 0u;
             __syncwarp();
             if (lane == 0) p8_arrive(&raw_full[stage]);
             now = next;
             next = after;
             ask(now);
         }
-    } else if (warp == 13) {
-        // ---- products ----
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = p8_idesc(P8_ROWS, P8_KEYS), idesc_o = p8_idesc(P8_ROWS, P8_D) | (1u << 16);      // V is MN-major
-            const uint32_t q_addr = tc_smem_u32(Qs), k_addr = tc_smem_u32(Ks), v_addr = tc_smem_u32(Vs);
-            const int last_t = n[1] > 0 ? 1 : 0;
-            // S of row tile t and key tile j; the first of the row tiles waits for the keys, the last frees them
-            auto scores = [&](int t, int j) {
-                if (t == 0 || j >= n[0]) mbar_wait(&k_full, j & 1, p.error_flag);
-                fa_fence_after();
-#pragma unroll
-                for (int k = 0; k < P8_D / 16; ++k) {
-                    const uint32_t off = (uint32_t)(k >> 2) * P8_HALF + (uint32_t)(k & 3) * 32;
-                    umma_f16(tmem + t * 128, umma_desc(q_addr + t * 2 * P8_HALF + off), umma_desc(k_addr + off), idesc_s, k != 0 ? 1u : 0u);
-                }
-                umma_commit(&s_full[t]);
-                if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&k_free);
-            };
-            for (int t = 0; t < 2; ++t)
-                if (n[t] > 0) scores(t, 0);
-            for (int j = 0; j < tiles; ++j) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (j >= n[t]) continue;
-                    mbar_wait(&p_full[t], j & 1, p.error_flag);
-                    if (t == 0 || j >= n[0]) mbar_wait(&v_full, j & 1, p.error_flag);
-                    fa_fence_after();
-#pragma unroll
-                    for (int k = 0; k < P8_KEYS / 16; ++k)       // 16 keys a product: 8 columns of P, 2 KB of V
-                        fa_umma_a_tmem(tmem + 256 + t * 128, tmem + t * 128 + k * 8, p8_desc_mn(v_addr + k * 2048), idesc_o, (j | k) != 0 ? 1u : 0u);
-                    umma_commit(&o_done[t]);
-                    if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&v_free);
-                    if (j + 1 < n[t]) scores(t, j + 1);
-                }
-            }
-        }
     } else if (warp >= 8) {
-        // ---- unpacking: a thread has a key ----
-        const int key = tid - 256;
-        const int from = (key / BOX) * 2 * BOX * P8_D + (key % BOX) * P8_D, to = key * 128;
+        // ---- unpacking ----
+        // Eight lanes take a key: lane c of them its entries 16 c .. 16 c + 15.
+        const int first = tid - 256, piece = first & 7, half = piece >> 2, at = (piece & 3) * 2;
         for (int j = 0; j < tiles; ++j) {
-            const unsigned char* src = raw + (j & 1) * P8_RAW_STAGE + from;
-            mbar_wait(&raw_full[j & 1], (j >> 1) & 1, p.error_flag);
-#pragma unroll
+            const unsigned char* src = raw + j % P8_STAGES * P8_RAW_STAGE;
+            const float2* of = scales[j % P8_SLOTS];
+            mbar_wait(&raw_full[j % P8_STAGES], j / P8_STAGES & 1, p.error_flag);
+            const int there = ctx - (t_begin + j) * P8_KEYS;     // keys of the tile that exist
+            const bool whole = there >= P8_KEYS && __all_sync(0xffffffffu, of[lane & 15].y > -INFINITY);
+#pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
-                if (j > 0) mbar_wait(kv == 0 ? &k_free : &v_free, (j - 1) & 1, p.error_flag);
-                unsigned char* dst = (kv == 0 ? Ks : Vs) + to;
-                // what is not there as zeros: it meets factors of zero
-                const bool there = kv == 0 || ((t_begin + j) * P8_KEYS + key < ctx && scales[j % P8_SCALE_SLOTS][key / 8].y > -INFINITY);
-                bool nan = false;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const uint4 four = *reinterpret_cast<const uint4*>(src + kv * BOX * P8_D + ((c ^ (key & 7)) << 4));
+                if (kv == 0 && j > 0) mbar_wait(&k_free, (j - 1) & 1, p.error_flag);
+                if (kv == 1 && j > 1) mbar_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, p.error_flag);
+                unsigned char* dst = (kv == 0 ? Ks : Vs + (j & 1) * 2 * P8_HALF) + half * P8_HALF;
+#pragma unroll 2
+                for (int key = first >> 3; key < P8_KEYS; key += P8_UNPACK * 4) {
+                    const uint4 four = *reinterpret_cast<const uint4*>(src + ((key / BOX) * 2 + kv) * BOX * P8_D + (key % BOX) * P8_D + ((piece ^ (key & 7)) << 4));
                     unsigned w[4] = {four.x, four.y, four.z, four.w};
-                    unsigned h[8];
+                    if (!whole && (key >= there || of[key / 8].y == -INFINITY)) w[0] = w[1] = w[2] = w[3] = 0u;      // not there: zeros, for factors of zero
+                    unsigned any = 0u, h[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (kv == 1) {
-                            if (!there) w[i] = 0u;
-                            const unsigned bad = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;         // bytes that are no number
-                            if (bad) {
-                                nan = true;
-                                w[i] &= ~((bad >> 7) * 0xffu);
-                            }
-                        }
-                        h[2 * i] = kv8_half2((unsigned short)w[i]);
-                        h[2 * i + 1] = kv8_half2((unsigned short)(w[i] >> 16));
+                        any |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;
+                        // a byte seeeemmm is s0eeeemmm0000000 in half precision, times 2^8; of four bytes the pairs 0, 2 and 1, 3
+                        h[2 * i] = ((w[i] << 7) & 0x3f803f80u) | ((w[i] << 8) & 0x80008000u);
+                        h[2 * i + 1] = ((w[i] >> 1) & 0x3f803f80u) | (w[i] & 0x80008000u);
                     }
-                    unsigned char* line = dst + (c >> 2) * P8_HALF;
-                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2) ^ (key & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + 1) ^ (key & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-                }
-                if (kv == 1) {
-                    const unsigned any = __ballot_sync(0xffffffffu, nan);
-                    if (lane == 0) no_number[j % P8_SCALE_SLOTS][warp - 8] = any;
+                    if (__builtin_expect(any & 0x80808080u, 0)) {        // what is no number: zeros as values, and the key is noted
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] &= ~(((((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
+                            h[2 * i] = ((w[i] << 7) & 0x3f803f80u) | ((w[i] << 8) & 0x80008000u);
+                            h[2 * i + 1] = ((w[i] >> 1) & 0x3f803f80u) | (w[i] & 0x80008000u);
+                        }
+                        atomicOr(&no_number[j % P8_SLOTS][key >> 5], 1u << (key & 31));
+                    }
+                    // (lanes of the second half of the head store their second piece first: the halves lie in the same banks)
+                    const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+                    *reinterpret_cast<uint4*>(dst + key * 128 + (((at + half) ^ (key & 7)) << 4)) = half ? hi : lo;
+                    *reinterpret_cast<uint4*>(dst + key * 128 + (((at + 1 - half) ^ (key & 7)) << 4)) = half ? lo : hi;
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    p8_arrive(kv == 0 ? &k_full : &v_full);
-                    if (kv == 1) p8_arrive(&raw_free[j & 1]);
-                }
+                if (lane == 0) p8_arrive(kv == 0 ? &k_full : &v_full[j & 1]);
             }
+            if (lane == 0) p8_arrive(&raw_free[j % P8_STAGES]);
         }
     } else {
         // ---- softmax ----
@@ -362,79 +399,70 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         const int pos_first = pos0 + tok0 + mine * P8_ROWS / G, pos_last = pos0 + tok0 + (min(rows, (mine + 1) * P8_ROWS) - 1) / G;
         float m = -INFINITY, mu = -INFINITY, l = 0.f;
         const int count = n[mine];
-        uint32_t a[32], b[32], pk[16];
+        uint32_t x[32], y[32], pk[16];
+        constexpr int BLOCK = BOX;
         for (int j = 0; j < count; ++j) {
-            const int j0 = (t_begin + j) * P8_KEYS, slot = j % P8_SCALE_SLOTS;
+            const int j0 = (t_begin + j) * P8_KEYS;
+            const float2* of = scales[j % P8_SLOTS];
             const bool mask = j0 + P8_KEYS - 1 > pos_first || (p.window > 0 && j0 < pos_last - p.window + 1) || rows < (mine + 1) * P8_ROWS;
-            const Tile8 tile{scales[slot], f, first - j0, pos - j0};
             mbar_wait(&s_full[mine], j & 1, p.error_flag);       // P V of the key tile before is done as well: it was issued before
             fa_fence_after();
             float t_top = -INFINITY, u_top = -INFINITY;
-            auto top = [&](const uint32_t (&x)[32], int col) {
-                if (mask) p8_top<true>(x, col, tile, t_top, u_top); else p8_top<false>(x, col, tile, t_top, u_top);
-            };
-            FA_TMEM_LD32(ts, a, 0);
-            fa_tmem_wait_ld();
-            FA_TMEM_LD32(ts + 32, b, 0);
-            top(a, 0);
-            fa_tmem_wait_ld();
-            FA_TMEM_LD32(ts + 64, a, 0);
-            top(b, 32);
-            fa_tmem_wait_ld();
-            FA_TMEM_LD32(ts + 96, b, 0);
-            top(a, 64);
-            fa_tmem_wait_ld();
-            FA_TMEM_LD32(ts, a, 0);                              // the first columns again
-            top(b, 96);
-            if (t_top > m + 8.f) {
+#pragma unroll 1
+            for (int c = 0; c < P8_KEYS; c += 64) {
+                FA_TMEM_LD32(ts + c, x, 0);
+                p8_wait_ld(x);
+                FA_TMEM_LD32(ts + c + 32, y, 0);
+                if (mask) fa_mask32(x, j0 + c, pos, first);
+                p8_top<BLOCK>(x, of + c / 8, f, t_top, u_top);
+                p8_wait_ld(y);
+                if (mask) fa_mask32(y, j0 + c + 32, pos, first);
+                p8_top<BLOCK>(y, of + c / 8 + 4, f, t_top, u_top);
+            }
+            if (t_top > m + 12.f) {
                 const float to_m = ceilf(t_top);
                 l *= m == -INFINITY ? 0.f : fa_ex2(m - to_m);
                 m = to_m;
             }
             float alpha = 1.f;
-            const bool raise = u_top > mu + 8.f;
+            const bool raise = u_top > mu + 12.f;
             if (raise) {
                 const float to_mu = ceilf(u_top);
                 alpha = fa_ex2(mu - to_mu);                      // 0 the first time
                 mu = to_mu;
             }
-            fa_tmem_wait_ld();
             if (j > 0 && __any_sync(0xffffffffu, raise)) {
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < P8_D; c += 32) {
-                    FA_TMEM_LD32(to + c, b, 0);
-                    fa_tmem_wait_ld();
+                    FA_TMEM_LD32(to + c, x, 0);
+                    p8_wait_ld(x);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) b[i] = __float_as_uint(__uint_as_float(b[i]) * alpha);
-                    FA_TMEM_ST32(to + c, b, 0);
+                    for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+                    FA_TMEM_ST32(to + c, x, 0);
                 }
             }
             const float m_now = m == -INFINITY ? 0.f : m, mu_now = mu == -INFINITY ? 0.f : mu;
-            auto factors = [&](const uint32_t (&x)[32], int col) {
-                if (mask) p8_factors<true>(x, col, tile, m_now, mu_now, pk, l); else p8_factors<false>(x, col, tile, m_now, mu_now, pk, l);
-            };
             // factors over the first 64 columns of S, always over columns that were read before
-            FA_TMEM_LD32(ts + 32, b, 0);
-            factors(a, 0);
-            fa_tmem_wait_ld();
-            FA_TMEM_LD32(ts + 64, a, 0);
-            FA_TMEM_ST16(ts, pk);
-            factors(b, 32);
-            fa_tmem_wait_ld();
-            FA_TMEM_LD32(ts + 96, b, 0);
-            FA_TMEM_ST16(ts + 16, pk);
-            factors(a, 64);
-            fa_tmem_wait_ld();
-            FA_TMEM_ST16(ts + 32, pk);
-            factors(b, 96);
-            FA_TMEM_ST16(ts + 48, pk);
+#pragma unroll 1
+            for (int c = 0; c < P8_KEYS; c += 64) {
+                FA_TMEM_LD32(ts + c, x, 0);
+                p8_wait_ld(x);
+                FA_TMEM_LD32(ts + c + 32, y, 0);
+                if (mask) fa_mask32(x, j0 + c, pos, first);
+                l += p8_factors<BLOCK>(x, of + c / 8, f, m_now, mu_now, pk);
+                p8_wait_ld(y);
+                FA_TMEM_ST16(ts + c / 2, pk);
+                if (mask) fa_mask32(y, j0 + c + 32, pos, first);
+                l += p8_factors<BLOCK>(y, of + c / 8 + 4, f, m_now, mu_now, pk);
+                FA_TMEM_ST16(ts + c / 2 + 16, pk);
+            }
             fa_tmem_wait_st();
             fa_fence_before();
             __syncwarp();
             if (lane == 0) p8_arrive(&p_full[mine]);
             // values that are no number: looked at once the tile's values are unpacked, which the next wait stands behind
             if (j > 0) {
-                const int before = (j - 1) % P8_SCALE_SLOTS, k0 = j0 - P8_KEYS;
+                const int before = (j - 1) % P8_SLOTS, k0 = j0 - P8_KEYS;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const unsigned bad = no_number[before][w];
@@ -447,7 +475,7 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         if (count > 0) mbar_wait(&o_done[mine], (count - 1) & 1, p.error_flag);
         fa_fence_after();
         if (count > 0) {
-            const int before = (count - 1) % P8_SCALE_SLOTS, k0 = (t_begin + count - 1) * P8_KEYS;
+            const int before = (count - 1) % P8_SLOTS, k0 = (t_begin + count - 1) * P8_KEYS;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const unsigned bad = no_number[before][w];
@@ -458,17 +486,24 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         }
         const float inv = l == 0.f ? 0.f : exp2f(mu - m) / l;    // no keys: zeros
         bf16* out = p.out + (size_t)(q_begin + tok0 + (live ? index / G : 0)) * p.out_stride + (size_t)(kvh * G + index % G) * P8_D;
+        uint32_t a[32];
         float* sums = p.partials + (((size_t)item.w * p.nkv + kvh) * (2 * P8_ROWS) + index) * P8_PART;
 #pragma unroll
         for (int c = 0; c < P8_D; c += 32) {
             if (count > 0) {
                 FA_TMEM_LD32(to + c, a, 0);
-                fa_tmem_wait_ld();
+                p8_wait_ld(a);
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) a[i] = 0u;
             }
             if (!live) continue;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {                    // columns 0, 2, 1, 3 of four, as the values are unpacked
+                const uint32_t swapped = a[i + 1];
+                a[i + 1] = a[i + 2];
+                a[i + 2] = swapped;
+            }
             if (parts == 1) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
@@ -488,7 +523,7 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
     }
     fa_fence_before();
     __syncthreads();
-    if (warp == 13) {
+    if (warp == 15) {
         fa_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -576,7 +611,7 @@ LLMP_API int llmp_kv8_prompt(const void* q, long q_stride, void* out, long out_s
     const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     LLMP_REQUIRE(rc == CUDA_SUCCESS, "kv8 prompt attention: cuTensorMapEncodeTiled failed with code %d", (int)rc);
-    const size_t smem = 8 * (size_t)P8_HALF + 2 * (size_t)P8_RAW_STAGE + 1024;
+    const size_t smem = 10 * (size_t)P8_HALF + P8_STAGES * (size_t)P8_RAW_STAGE + 1024;
     const auto kernel = box_tokens == 8 ? prompt_kv8_kernel<8> : box_tokens == 16 ? prompt_kv8_kernel<16> : prompt_kv8_kernel<32>;
     if (box_tokens == 8) LLMP_ALLOW_SMEM(prompt_kv8_kernel<8>, smem);
     else if (box_tokens == 16) LLMP_ALLOW_SMEM(prompt_kv8_kernel<16>, smem);

@@ -1,7 +1,7 @@
 """Attention of prompt portions over pages of 8-bit keys and values (``cache.spec.KV8PagesSpec``).
 
-bfloat16 queries of head size 128 have a kernel that reads the pages as they are (``kernels.kv8_prompt_attention``). For other
-sizes and for float32 the pages that a step's portions see are unpacked into a workspace of the query's type, laid out as ordinary
+Few bfloat16 queries of head size 128 over many keys go to a kernel that reads the pages as they are
+(``kernels.kv8_prompt_attention``; ``reads_pages_directly`` says when). For all others the pages that a step's portions see are unpacked into a workspace of the query's type, laid out as ordinary
 pages, and the attention kernels of ordinary pages run over it (``kernels.paged_attention``): a page's values are exact in
 either type (the scales are powers of two), so the result is exactly what they give for a cache that holds these values."""
 
@@ -19,21 +19,35 @@ KEY_TILE = 128                       # keys of a tile of the kernel that reads 8
 PART_TILES = 4
 
 
-def plan_items(starts: Sequence[int], q_lens: Sequence[int], first_request: int, tokens: int, num_kv_heads: int, window: int, sms: int,
-               most_places: int) -> Tuple[List[List[int]], List[List[int]], int]:
-    """(items, shared, places) for ``kernels.kv8_prompt_attention``: every ``tokens`` new tokens of a request are a tile, whose keys come
-    in parts where that evens out the work of ``sms`` SMs that run one item and key/value head at a time (few new tokens over many
-    keys). The items that see most keys come first."""
+def tiles_of(starts: Sequence[int], q_lens: Sequence[int], first_request: int, tokens: int, window: int) -> List[Tuple[int, int, int]]:
+    """(key tiles, request, first token) of every ``tokens`` new tokens of a request."""
     tiles = []
     for r in range(first_request, len(q_lens)):
         for t in range(0, q_lens[r], tokens):
             last = starts[r] + min(t + tokens, q_lens[r]) - 1
             low = max(starts[r] + t - window + 1, 0) if window else 0
             tiles.append((last // KEY_TILE + 1 - low // KEY_TILE, r, t))
-    share = max(PART_TILES, -(-sum(n for n, _r, _t in tiles) * num_kv_heads // sms))
-    parts = [-(-n // share) if n > 1.25 * share else 1 for n, _r, _t in tiles]
-    if sum(k for k in parts if k > 1) > most_places:
-        parts = [1] * len(tiles)
+    return tiles
+
+
+def plan_items(starts: Sequence[int], q_lens: Sequence[int], first_request: int, tokens: int, num_kv_heads: int, window: int, sms: int,
+               most_places: int) -> Tuple[List[List[int]], List[List[int]], int]:
+    """(items, shared, places) for ``kernels.kv8_prompt_attention``: every ``tokens`` new tokens of a request are a tile, whose keys come
+    in parts, as many as still give every part and key/value head an SM of its own (few new tokens over many keys). The items that
+    see most keys come first."""
+    tiles = tiles_of(starts, q_lens, first_request, tokens, window)
+    parts = [1] * len(tiles)
+    if tiles and len(tiles) * num_kv_heads <= sms:
+        low, high = PART_TILES, max(PART_TILES, max(n for n, _r, _t in tiles))
+        while low < high:                            # the fewest key tiles a part for which all parts run side by side
+            share = (low + high) // 2
+            if sum(-(-n // share) for n, _r, _t in tiles) * num_kv_heads <= sms:
+                high = share
+            else:
+                low = share + 1
+        parts = [-(-n // low) for n, _r, _t in tiles]
+        if sum(k for k in parts if k > 1) > most_places:
+            parts = [1] * len(tiles)
     items, shared, places = [], [], 0
     for i in sorted(range(len(tiles)), key=lambda i: (-tiles[i][0] / parts[i], tiles[i][1:])):
         _n, r, t = tiles[i]
@@ -43,6 +57,30 @@ def plan_items(starts: Sequence[int], q_lens: Sequence[int], first_request: int,
             shared.append([r, t, parts[i], places])
             places += parts[i]
     return items, shared, places
+
+
+def reads_pages_directly(starts: Sequence[int], q_lens: Sequence[int], first_request: int, num_heads: int, num_kv_heads: int, window: int,
+                         sms: int) -> bool:
+    """Whether a step's portions are better served by the kernel that reads 8-bit pages (256 query rows an item, its bytes unpacked in
+    every one) than by unpacking the pages once and the attention kernel of ordinary pages (128 rows, two of them on an SM; keys
+    shared by at most 8 items of at least 16 tiles). By what each takes, in us on a B200 (head size 128, 8 key/value heads):
+    18 and 4.5 a key tile of the longest part, against 8, 1.9 for every 1,000 tokens of the pages, and the longer of 2.8 a key tile
+    of the longest item and 2.2 for every key tile an SM has. Measured (direct, unpacked), 32 query heads: 40 new tokens behind 8,000
+    37, 70; 128 behind 2,000 33, 48; 256 behind 8,000 86, 85; 64 behind 500 26, 22; 2,048 new ones 86, 71; 2,048 behind 14,000 922, 604."""
+    group = num_heads // num_kv_heads
+    wide = tiles_of(starts, q_lens, first_request, max(1, 256 // group), window)
+    if not wide or len(wide) * num_kv_heads > sms:
+        return False
+    longest, places = 0, plan_items(starts, q_lens, first_request, max(1, 256 // group), num_kv_heads, window, sms, 1 << 30)[1]
+    cut = {(r, t): k for r, t, k, _p in places}
+    for n, r, t in wide:
+        longest = max(longest, -(-n // cut.get((r, t), 1)))
+    narrow = tiles_of(starts, q_lens, first_request, max(1, 128 // group), window)
+    blocks, most = len(narrow) * num_kv_heads, max(n for n, _r, _t in narrow)
+    segments = min(8, 4 * sms // blocks, most // 16) if blocks <= sms else 1
+    tokens = sum(s + n - (max(0, s - window + 1) if window else 0) for s, n in zip(starts[first_request:], q_lens[first_request:]) if n)
+    unpacked = 8 + 1.9e-3 * tokens * num_kv_heads / 8 + max(2.8 * -(-most // max(1, segments)), 2.2 * sum(n for n, _r, _t in narrow) * num_kv_heads / sms)
+    return 18 + 4.5 * longest < unpacked
 
 
 class PromptPlan:
@@ -67,6 +105,14 @@ class PromptPlan:
         self.groups = self._groups()
         self._lists: Dict[int, list] = {}            # by the width of the block tables
         self._items = None
+        self._direct = None
+
+    def direct(self) -> bool:
+        """Whether the portions go to the kernel that reads 8-bit pages (sizes it takes, and ``reads_pages_directly``)."""
+        if self._direct is None:
+            self._direct = kernels.kv8_prompt_supports(self.dtype, self.num_heads, self.num_kv_heads, self.head_dim, self.page_size) and \
+                reads_pages_directly(self.starts, self.q_lens, self.first_request, self.num_heads, self.num_kv_heads, self.window, kernels.sm_count())
+        return self._direct
 
     def pages_of(self, r: int) -> Tuple[int, int]:
         """The pages (first, end) of request r that its new tokens see."""
@@ -157,7 +203,7 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, q_stride: int, out: torc
         raise kernels.KernelError(f"a request sees {plan.longest} tokens, its block table has room for {block_tables.shape[1] * ps}")
     if not plan.groups:
         return out
-    if kernels.kv8_prompt_supports(q.dtype, nq, nkv, d, ps) and (q.data_ptr() | 2 * q_stride | out.data_ptr()) % 16 == 0:
+    if plan.direct() and (q.data_ptr() | 2 * q_stride | out.data_ptr()) % 16 == 0:
         items, shared, places = plan.items()
         return kernels.kv8_prompt_attention(q, q_stride, out, pages, block_tables, q_start, ctx_len, items, shared, places, nq, nkv, ps,
                                             plan.window, scale)

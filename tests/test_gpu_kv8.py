@@ -315,7 +315,8 @@ def test_single_tokens_in_a_page_pool_beyond_four_gigabytes():
     check_decode(host, torch.tensor([[0, 1, 2]]), q, ctx, nq, nkv, d, ps, 0, torch.bfloat16, out, d ** -0.5)
 
 
-def prompt(case, starts, lens, window, dtype, seed, first=0):
+def prompt(case, starts, lens, window, dtype, seed, first=0, direct=True):
+    """``direct``: through the kernel that reads 8-bit pages, where it takes the sizes."""
     from llm_pipeline_b200.ops import kv8
 
     nq, nkv, d, ps = case
@@ -328,6 +329,7 @@ def prompt(case, starts, lens, window, dtype, seed, first=0):
     q = torch.randn(N + 2, (nq + 2 * nkv) * d, generator=torch.Generator().manual_seed(seed)).to(dtype)
     out = torch.full((N + 2, nq * d), 9.0, dtype=dtype, device=DEV)
     plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, window, dtype, torch.device(DEV), first_request=first)
+    plan._direct = direct and K().kv8_prompt_supports(dtype, nq, nkv, d, ps)
     dev = dict(pages=host.raw.to(DEV), tables=tables.to(DEV), ctx=torch.tensor(ctx, dtype=torch.int32, device=DEV), q=q.to(DEV),
                start=torch.tensor([sum(lens[:r]) for r in range(len(lens) + 1)], dtype=torch.int32, device=DEV))
     kv8.prompt_attention(plan, dev["q"], q.stride(0), out, dev["pages"], dev["tables"], dev["start"], dev["ctx"], d ** -0.5)
@@ -340,10 +342,11 @@ PORTIONS = [([0], [1]), ([0], [300]), ([37, 0, 500], [129, 1, 70]), ([1000, 3], 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("window", [0, 50])
 @pytest.mark.parametrize("portions", range(len(PORTIONS)))
+@pytest.mark.parametrize("direct", [True, False])
 @pytest.mark.parametrize("nq,nkv,d,ps", [(32, 8, 128, 16), (6, 2, 80, 8), (5, 5, 48, 4), (9, 1, 128, 64)])
-def test_prompt_portions(dtype, nq, nkv, d, ps, portions, window):
+def test_prompt_portions(dtype, nq, nkv, d, ps, direct, portions, window):
     starts, lens = PORTIONS[portions]
-    host, tables, ctx, q, out = prompt((nq, nkv, d, ps), starts, lens, window, dtype, 31 + portions)
+    host, tables, ctx, q, out = prompt((nq, nkv, d, ps), starts, lens, window, dtype, 31 + portions, direct=direct)
     at = 0
     for r, n in enumerate(lens):
         rows = sorted({0, 1, n // 2, n - 1} & set(range(n)))
@@ -405,6 +408,7 @@ def test_prompt_portions_over_blocks_of_very_different_scales():
     q = q.bfloat16()
     out = torch.full((250, nq * d), 9.0, dtype=torch.bfloat16, device=DEV)
     plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, 0, torch.bfloat16, torch.device(DEV))
+    plan._direct = True
     kv8.prompt_attention(plan, q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), torch.tensor([0, 100, 250], dtype=torch.int32, device=DEV),
                          torch.tensor(ctx, dtype=torch.int32, device=DEV), d ** -0.5)
     check_prompt(host, tables, ctx, q, out, starts, lens, nq, nkv, d, 0)
@@ -424,6 +428,7 @@ def test_what_a_row_cannot_see_does_not_matter_to_it(dim, ps):
     q[5, 3 * dim] = float("nan")
     out = torch.full_like(clean, 9.0)
     plan = kv8.PromptPlan(starts, lens, nq, nkv, dim, ps, window, torch.bfloat16, torch.device(DEV))
+    plan._direct = True
     kv8.prompt_attention(plan, q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), torch.tensor([0, 300], dtype=torch.int32, device=DEV),
                          torch.tensor(ctx, dtype=torch.int32, device=DEV), dim ** -0.5)
     nan = out[:300].view(300, nq, dim).isnan()
@@ -441,12 +446,17 @@ def test_prompt_portions_in_turns_of_a_small_workspace(monkeypatch):
     from llm_pipeline_b200.ops import kv8
 
     case, starts, lens = (32, 8, 128, 16), [37, 0, 500, 20], [129, 1, 70, 33]
-    whole = prompt(case, starts, lens, 0, torch.bfloat16, 41)[-1]
+    whole = prompt(case, starts, lens, 0, torch.bfloat16, 41, direct=False)[-1]
+    direct = prompt(case, starts, lens, 0, torch.bfloat16, 41, first=2)[-1]
     monkeypatch.setattr(kv8, "WORKSPACE_BYTES", 1 << 20)
-    assert torch.equal(prompt(case, starts, lens, 0, torch.bfloat16, 41)[-1], whole)
+    assert torch.equal(prompt(case, starts, lens, 0, torch.bfloat16, 41, direct=False)[-1], whole)
     # the first requests left to another kernel
-    part = prompt(case, starts, lens, 0, torch.bfloat16, 41, first=2)[-1]
+    part = prompt(case, starts, lens, 0, torch.bfloat16, 41, first=2, direct=False)[-1]
     assert bool((part[:130] == 9).all()) and torch.equal(part[130:], whole[130:])
+    assert bool((direct[:130] == 9).all()) and not bool((direct[130:-2] == 9).any())
+    # without places for sums the kernel that reads 8-bit pages takes every tile's keys whole (other sums, so by the plain form)
+    host, tables, ctx, q, out = prompt(case, starts, lens, 0, torch.bfloat16, 41)
+    check_prompt(host, tables, ctx, q, out, starts, lens, 32, 8, 128, 0)
 
 
 def test_a_step_in_a_graph_and_on_two_streams():

@@ -131,3 +131,33 @@ def test_a_model_without_such_layers_refuses():
 
     with pytest.raises(ValueError, match="8 bits"):
         build_model(resolve_config(Z.CONFIGS["wkv_only"])).cache_specs("e4m3")
+
+
+def test_items_cover_every_key_tile_of_every_token_once():
+    import random
+
+    rng = random.Random(1)
+    for _ in range(200):
+        R = rng.randint(1, 5)
+        starts, lens = [rng.choice([0, rng.randint(0, 9000)]) for _ in range(R)], [rng.choice([0, 1, rng.randint(1, 2000)]) for _ in range(R)]
+        tokens, window, first, nkv = rng.choice([64, 128, 32, 256]), rng.choice([0, 0, 50, 1000]), rng.randint(0, R), rng.choice([1, 8])
+        items, shared, places = kv8.plan_items(starts, lens, first, tokens, nkv, window, 148, rng.choice([0, 100, 10000]))
+        seen, used = set(), set()
+        for r, t, x, place in items:
+            part, parts = x & 0xffff, x >> 16
+            tiles = dict(((a, b), n) for n, a, b in kv8.tiles_of(starts, lens, first, tokens, window))[r, t]
+            assert 0 <= part < parts <= tiles and (r, t, part) not in seen
+            seen.add((r, t, part))
+            if parts > 1:
+                assert place not in used
+                used.add(place)
+        assert {(r, t) for r, t, _part in seen} == {(r, t) for r in range(first, R) for t in range(0, lens[r], tokens)}
+        assert used == set(range(places)) and sum(s[2] for s in shared) == places
+        if any(x >> 16 > 1 for _r, _t, x, _p in items):
+            assert len(items) * nkv <= 148
+
+
+def test_which_kernel_portions_take():
+    take = lambda starts, lens, nq=32: kv8.reads_pages_directly(starts, lens, 0, nq, 8, 0, 148)         # noqa: E731
+    assert take([8003], [40]) and take([2000], [128]) and take([2000], [8])
+    assert not take([0], [2048]) and not take([14000], [2048]) and not take([500], [64]) and not take([], []) and not take([5], [0])
