@@ -8,9 +8,11 @@ tensor that is not on a CUDA device is an error.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import math
+import operator
 import os
 from typing import Optional, Sequence, Tuple
 
@@ -2309,24 +2311,27 @@ def wkv_gate(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, out: tor
 # (Steps of single tokens make these calls for every layer: messages are made only where they are raised.)
 def _on_current_device(*tensors: torch.Tensor) -> None:
     """Kernels run on the current device: an error for a tensor that is anywhere else."""
-    here = None
+    here = _device() if tensors[0].get_device() >= 0 else -1
     for t in tensors:
-        at = t.get_device()
-        if at < 0:
-            raise KernelError("a kernel was given a tensor that is not on a CUDA device; this engine has no CPU path")
-        if here is None:
-            here = _device()
-        if at != here:
-            raise KernelError(f"a tensor is on cuda:{at}, the current device is cuda:{here}")
+        if t.get_device() != here or here < 0:
+            if t.get_device() < 0:
+                raise KernelError("a kernel was given a tensor that is not on a CUDA device; this engine has no CPU path")
+            raise KernelError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{_device()}")
 
 
-def _kv8_pages(pages: torch.Tensor, num_kv_heads: int, head_dim: int, page_size: int) -> None:
+@functools.lru_cache(maxsize=None)
+def _kv8_page_bytes(num_kv_heads: int, head_dim: int, page_size: int) -> int:
     if not (num_kv_heads > 0 and page_size > 0 and 16 <= head_dim <= 256 and head_dim % 16 == 0):
         raise KernelError("8-bit pages take head sizes that are multiples of 16 in 16..256, and at least one head and token")
-    if not (pages.dtype == torch.uint8 and pages.dim() == 2 and pages.is_contiguous() and pages.shape[0] > 0 and
-            pages.shape[1] == kv8_page_bytes(num_kv_heads, page_size, head_dim)):
-        raise KernelError(f"8-bit pages must be contiguous uint8 [pages, {kv8_page_bytes(num_kv_heads, page_size, head_dim)}] for {num_kv_heads} "
-                          f"heads of {head_dim} and {page_size} tokens")
+    return kv8_page_bytes(num_kv_heads, page_size, head_dim)
+
+
+def _kv8_pages(pages: torch.Tensor, num_kv_heads: int, head_dim: int, page_size: int) -> int:
+    """Checks 8-bit pages; how many they are."""
+    size, shape = _kv8_page_bytes(num_kv_heads, head_dim, page_size), pages.shape
+    if len(shape) != 2 or shape[1] != size or shape[0] == 0 or pages.dtype != torch.uint8 or not pages.is_contiguous():
+        raise KernelError(f"8-bit pages must be contiguous uint8 [pages, {size}] for {num_kv_heads} heads of {head_dim} and {page_size} tokens")
+    return shape[0]
 
 
 def kv8_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor, num_kv_heads: int, head_dim: int,
@@ -2336,16 +2341,17 @@ def kv8_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torc
     neighbours, in the order of the tokens (as a step's rows are). Each head's keys, and values, of a page share a scale, the
     smallest power of two that holds them; storing behind a page's first token raises the scale where that is needed and
     moves what the page holds up to there to it. A row at offset 0 starts its page anew. Infinities and NaN are held as NaN."""
-    _kv8_pages(pages, num_kv_heads, head_dim, page_size)
+    P = _kv8_pages(pages, num_kv_heads, head_dim, page_size)
     _i32(slots, "slots")
-    N = slots.numel()
-    if not (k.dim() == 2 and k.shape == (N, num_kv_heads * head_dim) and v.shape == k.shape and k.dtype == v.dtype):
+    N, shape, kind = slots.numel(), k.shape, k.dtype
+    if shape != (N, num_kv_heads * head_dim) or v.shape != shape or v.dtype != kind:
         raise KernelError("keys and values must be [tokens, kv heads * head_dim] of one type, one row per slot")
-    if N > 1 and not (k.stride(1) == 1 and v.stride(1) == 1):
+    k_stride, v_stride = k.stride(), v.stride()
+    if N > 0 and (k_stride[1] != 1 or v_stride[1] != 1):
         raise KernelError("the entries of a row of keys or values must be neighbours")
-    dtype = dtype_code(k.dtype)
+    dtype = dtype_code(kind)
     _on_current_device(k, v, slots, pages)
-    _call("llmp_kv8_store", k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), dtype, slots.data_ptr(), pages.data_ptr(), pages.shape[0], N,
+    _call("llmp_kv8_store", k.data_ptr(), k_stride[0], v.data_ptr(), v_stride[0], dtype, slots.data_ptr(), pages.data_ptr(), P, N,
           num_kv_heads, head_dim, page_size, _stream())
 
 
@@ -2353,24 +2359,26 @@ def kv8_gather(pages: torch.Tensor, block_tables: torch.Tensor, ctx_len: torch.T
     """out[i] (``[n, 2, kv heads, page_size, head_dim]``, float32 or bfloat16, exact in either) = the values of the 8-bit page
     that entry ``index[i]`` of the flattened ``block_tables`` names; zeros behind the request's last token and for a page that
     is missing."""
-    if not (out.dim() == 5 and out.shape[1] == 2 and out.is_contiguous()):
+    shape, table = out.shape, block_tables.shape
+    if len(shape) != 5 or shape[1] != 2 or not out.is_contiguous():
         raise KernelError("unpacked pages must be contiguous [n, 2, kv heads, page_size, head_dim]")
-    n, _two, nkv, page_size, d = out.shape
-    _kv8_pages(pages, nkv, d, page_size)
+    n, _two, nkv, page_size, d = shape
+    P = _kv8_pages(pages, nkv, d, page_size)
     _i32(block_tables, "block_tables")
     _i32(ctx_len, "ctx_len")
     _i32(index, "index")
-    if block_tables.dim() != 2 or block_tables.shape[0] != ctx_len.numel():
+    if len(table) != 2 or table[0] != ctx_len.numel():
         raise KernelError("block tables must be [requests, pages]")
     if index.numel() != n:
         raise KernelError("one index per unpacked page")
     dtype = dtype_code(out.dtype)
     _on_current_device(pages, block_tables, ctx_len, index, out)
-    _call("llmp_kv8_gather", pages.data_ptr(), pages.shape[0], block_tables.data_ptr(), ctx_len.numel(), block_tables.shape[1], ctx_len.data_ptr(),
+    _call("llmp_kv8_gather", pages.data_ptr(), P, block_tables.data_ptr(), table[0], table[1], ctx_len.data_ptr(),
           index.data_ptr(), n, out.data_ptr(), dtype, nkv, d, page_size, _stream())
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def kv8_decode_scratch_floats(rows: int, num_heads: int, head_dim: int, max_ctx: int) -> int:
     fn = library().llmp_kv8_decode_scratch_floats
     fn.argtypes = [_I, _I, _I, _I]
@@ -2393,6 +2401,7 @@ def _kv8_stream_sizes() -> Tuple[int, int]:
 
 
 _kv8_workspaces: dict = {}
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)     # (without the set-up check around it)
 KV8_CAPTURED_CALLS = 4096                        # captured calls with counters from the slab
 
 
@@ -2401,7 +2410,7 @@ def kv8_workspace(device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
     another and share a pair. A captured call gets a pair of its own, since its graph may be replayed beside others: counters from a
     slab that was made outside a capture, or, where there is none or it is used up, counters that the graph itself zeroes."""
     here = _device()
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         floats, count = _kv8_stream_sizes()
         scratch = torch.empty(floats, dtype=torch.float32, device=device)
         slab = _kv8_workspaces.get((here, "slab"))
@@ -2426,34 +2435,34 @@ def kv8_decode_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
     """Attention of one query row per request (row r belongs to request r, at position ctx_len[r] - 1) over the request's 8-bit
     pages, as ``decode_attention`` over pages of q's type. No context is longer than ``max_ctx``. A request without keys gets zeros;
     a page that is missing from the tables has no keys; what lies behind the context or before the window never matters."""
-    _kv8_pages(pages, num_kv_heads, head_dim, page_size)
+    P = _kv8_pages(pages, num_kv_heads, head_dim, page_size)
     _i32(block_tables, "block_tables")
     _i32(ctx_len, "ctx_len")
-    R, width = ctx_len.numel(), num_heads * head_dim
+    R, width, kind = ctx_len.numel(), num_heads * head_dim, q.dtype
     if num_heads <= 0 or num_heads % num_kv_heads:
         raise KernelError(f"{num_heads} query heads cannot share {num_kv_heads} key/value heads")
-    if not (q.dtype == out.dtype and q.dim() == 2 and q.shape[0] >= R and q.shape[1] >= width and q.stride(1) == 1 and
-            (R <= 1 or q.stride(0) == q_stride)):
+    shape, stride, table = q.shape, q.stride(), block_tables.shape
+    if len(shape) != 2 or shape[0] < R or shape[1] < width or stride[1] != 1 or (R > 1 and stride[0] != q_stride) or out.dtype != kind:
         raise KernelError("query rows must be [requests, at least heads * head_dim] of the output's type")
-    if not (out.is_contiguous() and out.shape == (R, width)):
+    if out.shape != (R, width) or not out.is_contiguous():
         raise KernelError("decode output must be [requests, heads * head_dim]")
-    if not (block_tables.dim() == 2 and block_tables.shape[0] == R and block_tables.shape[1] > 0):
+    if len(table) != 2 or table[0] != R or table[1] == 0:
         raise KernelError("block tables must be [requests, pages]")
     if max_ctx <= 0 or window < 0:
         raise KernelError("the longest context must be positive, a window not negative")
-    dtype = dtype_code(q.dtype)
+    dtype = dtype_code(kind)
     _on_current_device(q, out, pages, block_tables, ctx_len)
-    at = q.data_ptr()
-    if kv8_stream_supports(q.dtype, num_heads, num_kv_heads, head_dim, page_size) and (at | 2 * q_stride) % 16 == 0 and out.data_ptr() % 8 == 0:
+    at, to = q.data_ptr(), out.data_ptr()
+    if kv8_stream_supports(kind, num_heads, num_kv_heads, head_dim, page_size) and (at | 2 * q_stride) % 16 == 0 and to % 8 == 0:
         scratch, counters = kv8_workspace(q.device)
-        _call("llmp_kv8_stream", at, q_stride, out.data_ptr(), width, pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
-              block_tables.shape[1], ctx_len.data_ptr(), R, max_ctx, num_heads, num_kv_heads, page_size, window, scale, scratch.data_ptr(),
-              scratch.numel(), counters.data_ptr(), error_flag().data_ptr(), _stream())
+        _call("llmp_kv8_stream", at, q_stride, to, width, pages.data_ptr(), P, block_tables.data_ptr(), table[1], ctx_len.data_ptr(), R, max_ctx,
+              num_heads, num_kv_heads, page_size, window, scale, scratch.data_ptr(), scratch.numel(), counters.data_ptr(),
+              error_flag().data_ptr(), _stream())
         return out
-    scratch = torch.empty(kv8_decode_scratch_floats(R, num_heads, head_dim, max_ctx), dtype=torch.float32, device=q.device)
-    _call("llmp_kv8_decode", at, q_stride, out.data_ptr(), width, dtype, pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
-          block_tables.shape[1], ctx_len.data_ptr(), R, max_ctx, num_heads, num_kv_heads, head_dim, page_size, window, scale, scratch.data_ptr(),
-          scratch.numel(), _stream())
+    floats = kv8_decode_scratch_floats(R, num_heads, head_dim, max_ctx)
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+    _call("llmp_kv8_decode", at, q_stride, to, width, dtype, pages.data_ptr(), P, block_tables.data_ptr(), table[1], ctx_len.data_ptr(), R, max_ctx,
+          num_heads, num_kv_heads, head_dim, page_size, window, scale, scratch.data_ptr(), floats, _stream())
     return out
 
 
@@ -2497,35 +2506,50 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     """tensor[dst[i]] = tensor[src[i]] for every i in each of the ``tensors`` (contiguous, one size of page, as many pages at
     least as the numbers ask for), in one launch for as many as its parameters take. No destination may be a source or twice
     a destination: the copies have no order."""
-    if len(src) != len(dst):
+    n = len(src)
+    if n != len(dst):
         raise KernelError("as many destinations as sources are needed")
-    if not len(tensors) or not len(src):
+    tensors = list(tensors)
+    if not tensors or not n:
         return
-    pairs = np.array([src, dst], dtype=np.int32)
-    first = tensors[0]
-    shape, kind = first.shape[1:], first.dtype
-    pages = first.shape[0] if first.dim() else 0
-    for t in tensors:
-        if not (t.dim() >= 1 and t.is_contiguous() and t.dtype == kind and t.shape[1:] == shape):
+    # (a fork copies a page in every layer: what is asked of all caches is asked in C loops)
+    first, shapes = tensors[0], list(map(_shape_of, tensors))
+    shape, pages = shapes[0], shapes[0][0] if shapes[0] else 0
+    if shapes.count(shape) != len(shapes):                       # pools of different sizes: of one page all the same
+        if not all(s and s[1:] == shape[1:] for s in shapes):
             raise KernelError("the caches of a copy must be contiguous, of one page size and one type")
-        if t.shape[0] < pages:
-            pages = t.shape[0]
-    if int(pairs.min()) < 0 or int(pairs.max()) >= pages:
+        pages = min(s[0] for s in shapes)
+    if not all(map(torch.Tensor.is_contiguous, tensors)) or len(set(map(_dtype_of, tensors))) != 1 or not shape:
+        raise KernelError("the caches of a copy must be contiguous, of one page size and one type")
+    src, dst = array.array("i", src), array.array("i", dst)
+    if n <= 64:                                                  # (8 pages: 21 us a call, through numpy 37; 1,500: 245 and 105)
+        low, high, to = min(min(src), min(dst)), max(max(src), max(dst)), set(dst)
+        clash = len(to) != n or not to.isdisjoint(src)
+    else:
+        a, b = np.frombuffer(src, dtype=np.int32), np.frombuffer(dst, dtype=np.int32)
+        low, high = min(int(a.min()), int(b.min())), max(int(a.max()), int(b.max()))
+        clash = False
+        if low >= 0 and high < pages:
+            role = np.bincount(b, minlength=pages)               # how often a page is a destination
+            clash = int(role.max()) > 1 or bool(role[a].any())
+    if low < 0 or high >= pages:
         raise KernelError(f"a page to copy is outside 0..{pages - 1}")
-    role = np.zeros(pages, dtype=np.int32)                       # 1 per time a page is a destination, and a source
-    np.add.at(role, pairs[1], 1)
-    role[pairs[0]] += 1
-    if int(role[pairs[1]].max()) > 1:
+    if clash:
         raise KernelError("a page is twice a destination, or a source and a destination")
-    _on_current_device(*tensors)
-    page_bytes = math.prod(shape) * first.element_size()
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if len(devices) != 1 or -1 in devices or _device() not in devices:
+        _on_current_device(*tensors)
+    page_bytes = math.prod(shape[1:]) * first.element_size()
     most_tensors, most_pairs = _copy_pages_sizes()
-    pointers = [t.data_ptr() for t in tensors]
+    pointers = list(map(torch.Tensor.data_ptr, tensors))
     for at in range(0, len(pointers), most_tensors):
-        bases = (_P * len(pointers[at:at + most_tensors]))(*pointers[at:at + most_tensors])
-        for i in range(0, len(src), most_pairs):
-            n = min(most_pairs, len(src) - i)
-            _call("llmp_copy_pages", bases, len(bases), page_bytes, pairs.ctypes.data + 4 * i, pairs.ctypes.data + 4 * (len(src) + i), n, _stream())
+        bases = array.array("Q", pointers[at:at + most_tensors])
+        for i in range(0, n, most_pairs):
+            _call("llmp_copy_pages", bases.buffer_info()[0], len(bases), page_bytes, src.buffer_info()[0] + 4 * i, dst.buffer_info()[0] + 4 * i,
+                  min(most_pairs, n - i), _stream())
+
+
+_shape_of, _dtype_of = operator.attrgetter("shape"), operator.attrgetter("dtype")
 
 
 @functools.lru_cache(maxsize=None)

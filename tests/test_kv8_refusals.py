@@ -72,6 +72,15 @@ def test_copy_pages(tensors, src, dst, message):
         kernels.copy_pages(tensors, src, dst)
 
 
+def test_copy_pages_of_many():
+    t = torch.zeros(400, 3)
+    for src, dst, message in (([0] * 100, list(range(1, 100)) + [400], "outside"), ([0] * 100, [-1] + list(range(1, 100)), "outside"),
+                              ([0] * 100, [5] * 2 + list(range(6, 104)), "twice"), (list(range(100)), list(range(99, 199)), "twice"),
+                              (list(range(100)), list(range(100, 200)), "not on a CUDA device")):
+        with pytest.raises(kernels.KernelError, match=message):
+            kernels.copy_pages([t], src, dst)
+
+
 def test_nothing_to_copy():
     kernels.copy_pages([], [1], [2])
     kernels.copy_pages([torch.zeros(4, 3)], [], [])
