@@ -7,7 +7,7 @@ either type (the scales are powers of two), so the result is exactly what they g
 
 from __future__ import annotations
 
-from typing import Dict, List, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -87,7 +87,8 @@ class PromptPlan:
     """What a step's prompt attention needs besides its tensors. One plan serves every layer of a step with the same heads, head size,
     page size and window. ``starts`` and ``q_lens``: cached tokens and new tokens of every request, as host numbers; the requests
     before ``first_request`` are left out (their rows of the output are not written). Its lists are made on the stream that is
-    current when it is first used."""
+    current when it is first used; a call on another stream waits for that one. A captured call needs a plan that was used before with
+    tables of the same width, and the plan has to live as long as the graph."""
 
     def __init__(self, starts: Sequence[int], q_lens: Sequence[int], num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                  window: int, dtype: torch.dtype, device: torch.device, first_request: int = 0):
@@ -106,10 +107,11 @@ class PromptPlan:
         self._lists: Dict[int, list] = {}            # by the width of the block tables
         self._items = None
         self._direct = None
+        self._made: Optional[torch.cuda.Stream] = None          # the stream the lists were made on
 
     def direct(self) -> bool:
         """Whether the portions go to the kernel that reads 8-bit pages (sizes it takes, and ``reads_pages_directly``)."""
-        if self._direct is None:
+        if self._direct is None:                     # (asked once a plan, that is once a step)
             self._direct = kernels.kv8_prompt_supports(self.dtype, self.num_heads, self.num_kv_heads, self.head_dim, self.page_size) and \
                 reads_pages_directly(self.starts, self.q_lens, self.first_request, self.num_heads, self.num_kv_heads, self.window, kernels.sm_count())
         return self._direct
@@ -137,12 +139,28 @@ class PromptPlan:
 
     def _on_device(self, lists: Sequence[torch.Tensor]) -> List[torch.Tensor]:
         """The int32 lists through one pinned copy, each from a multiple of 16 bytes on."""
+        if kernels._capturing():
+            raise kernels.KernelError("a plan's lists must exist before a graph is captured: call it once with this step's tables before")
         padded = [torch.nn.functional.pad(t.flatten(), (0, -t.numel() % 4)) for t in lists]
+        stream = torch.cuda.current_stream(self.device)
+        if self._made is not None and self._made != stream:
+            stream.wait_stream(self._made)           # this stream's work then comes behind all lists, whichever it waits for later
+        self._made = stream
         dev, at, out = torch.cat(padded).pin_memory().to(self.device, non_blocking=True), 0, []
         for t, room in zip(lists, padded):
             out.append(dev[at:at + t.numel()].view(t.shape))
             at += room.numel()
         return out
+
+    def _for_this_stream(self, lists: Sequence[Optional[torch.Tensor]]) -> None:
+        """Before work on another stream than the lists' own: it comes behind them, and their memory is not given away before its end."""
+        if kernels._stream() == self._made.cuda_stream or kernels._capturing():      # (a capture begins with an idle device)
+            return
+        stream = torch.cuda.current_stream(self.device)
+        stream.wait_stream(self._made)
+        for t in lists:
+            if t is not None:
+                t.record_stream(stream)
 
     def items(self):
         """(items, shared, places) on the device for the kernel that reads 8-bit pages."""
@@ -201,14 +219,18 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, q_stride: int, out: torc
         raise kernels.KernelError("the plan has more rows than the queries or the output")
     if block_tables.shape[1] * ps < plan.longest:
         raise kernels.KernelError(f"a request sees {plan.longest} tokens, its block table has room for {block_tables.shape[1] * ps}")
+    if not 0.0 < scale < float("inf"):                 # both ways take a row's largest score before they scale it
+        raise kernels.KernelError(f"the scale of a prompt's scores must be positive and finite, not {scale}")
     if not plan.groups:
         return out
     if plan.direct() and (q.data_ptr() | 2 * q_stride | out.data_ptr()) % 16 == 0:
         items, shared, places = plan.items()
+        plan._for_this_stream((items, shared))
         return kernels.kv8_prompt_attention(q, q_stride, out, pages, block_tables, q_start, ctx_len, items, shared, places, nq, nkv, ps,
                                             plan.window, scale)
     kernels._on_current_device(q, out, pages, block_tables, q_start, ctx_len)
     for index, tables, req, tok0, seg, slot, places, tokens in plan.lists(block_tables.shape[1]):
+        plan._for_this_stream((index, tables, req, tok0, seg, slot))
         held = torch.empty((index.numel(), 2, nkv, ps, d), dtype=q.dtype, device=q.device)
         kernels.kv8_gather(pages, block_tables, ctx_len, index, held)
         kernels.paged_attention(q, q_stride, out, held, tables, q_start, ctx_len, req, tok0, nq, nkv, d, ps, plan.window, scale, tokens,

@@ -294,6 +294,68 @@ def test_single_tokens_with_sharp_and_flat_scores(dtype, nq, nkv, d, ps):
     assert torch.equal(out.view(2, nq, d)[~nan], clean.view(2, nq, d)[~nan])
 
 
+def test_more_requests_than_a_launch_takes_and_a_negative_scale():
+    """700 requests: two launches of the streaming kernel on one set of counters; scores with their signs turned, and of no size at all."""
+    nq, nkv, d, ps = 8, 2, 128, 16
+    ctx = [(37 * r) % 90 for r in range(700)]
+    host, tables, q = decode_case(nq, nkv, d, ps, ctx, torch.bfloat16, 17)
+    spoil(host, tables, ctx, ps)
+    for scale in (-0.1, 0.0, 0.09):
+        out = torch.full((700, nq * d), 9.0, dtype=torch.bfloat16, device=DEV)
+        K().kv8_decode_attention(q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV), 90, nq, nkv,
+                                 d, ps, 0, scale)
+        for r in (0, 1, 2, 300, 511, 512, 513, 600, 699):
+            k, v, there = host.request(tables[r], ctx[r])
+            want, size, top = plain.attend(q[r:r + 1, :nq * d].view(1, nq, d), k, v, [ctx[r] - 1], there, scale, 0)
+            assert bool(((out[r].double().cpu().view(1, nq, d) - want).abs() <= bound(want, size, top.abs(), torch.bfloat16, d)).all()), (scale, r)
+
+
+def test_portions_captured_and_replayed():
+    """A plan that has been used is captured; one that has not is refused inside a capture, and the stream goes on."""
+    from llm_pipeline_b200.ops import kernels, kv8
+
+    nq, nkv, d, ps, starts, lens = 32, 8, 128, 16, [3000], [40]
+    for direct in (True, False):
+        host, tables, ctx, q, want = prompt((nq, nkv, d, ps), starts, lens, 0, torch.bfloat16, 95, direct=direct)
+        dev = [q.to(DEV), host.raw.to(DEV), tables.to(DEV), torch.tensor([0, 40], dtype=torch.int32, device=DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV)]
+        out = torch.full_like(want, 9.0)
+        plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, 0, torch.bfloat16, torch.device(DEV))
+        plan._direct = direct
+        call = lambda p: kv8.prompt_attention(p, dev[0], q.stride(0), out, dev[1], dev[2], dev[3], dev[4], d ** -0.5)       # noqa: E731
+        call(plan)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(plan)
+            fresh = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, 0, torch.bfloat16, torch.device(DEV))
+            fresh._direct = direct
+            with pytest.raises(kernels.KernelError, match="before a graph"):
+                call(fresh)
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("direct", [True, False])
+def test_one_plan_on_two_streams(direct):
+    from llm_pipeline_b200.ops import kv8
+
+    nq, nkv, d, ps, starts, lens = 32, 8, 128, 16, [500, 0], [40, 9]
+    host, tables, ctx, q, want = prompt((nq, nkv, d, ps), starts, lens, 0, torch.bfloat16, 96, direct=direct)
+    dev = [q.to(DEV), host.raw.to(DEV), tables.to(DEV), torch.tensor([0, 40, 49], dtype=torch.int32, device=DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV)]
+    plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, 0, torch.bfloat16, torch.device(DEV))
+    plan._direct = direct
+    torch.cuda.synchronize()
+    outs = []
+    for stream in (torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.current_stream()):
+        with torch.cuda.stream(stream):
+            outs.append(torch.full((49, nq * d), 9.0, dtype=torch.bfloat16, device=DEV))
+            kv8.prompt_attention(plan, dev[0], q.stride(0), outs[-1], dev[1], dev[2], dev[3], dev[4], d ** -0.5)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[:49]) for out in outs)
+
+
 def test_single_tokens_in_a_page_pool_beyond_four_gigabytes():
     """Pages whose bytes begin beyond 32-bit offsets."""
     nq, nkv, d, ps = 32, 8, 128, 64

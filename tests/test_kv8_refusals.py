@@ -104,6 +104,10 @@ def test_plans():
     with pytest.raises(kernels.KernelError, match="more rows"):
         kv8.prompt_attention(plan, torch.zeros(20, 4 * D), 4 * D, torch.zeros(21, 4 * D), pages(), torch.zeros(3, 15, dtype=torch.int32), i32(0, 20, 20, 21),
                              i32(120, 0, 8), 1.0)
+    for scale in (0.0, -0.5, float("nan"), float("inf")):
+        with pytest.raises(kernels.KernelError, match="positive and finite"):
+            kv8.prompt_attention(plan, torch.zeros(21, 4 * D), 4 * D, torch.zeros(21, 4 * D), pages(), torch.zeros(3, 15, dtype=torch.int32),
+                                 i32(0, 20, 20, 21), i32(120, 0, 8), scale)
 
 
 def test_the_workspace_holds_a_few_requests_at_a_time(monkeypatch):
