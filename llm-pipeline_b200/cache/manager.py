@@ -28,9 +28,11 @@ from .spec import PagesSpec, StateSpec
 
 
 def copy_pages(tensors, src, dst) -> None:
+    """On the current stream of the caches' device, which need not be the current one."""
     from ..ops import kernels
 
-    kernels.copy_pages(tensors, src, dst)
+    with torch.cuda.device_of(tensors[0]):
+        kernels.copy_pages(tensors, src, dst)
 
 
 class CacheError(RuntimeError):
@@ -336,8 +338,9 @@ class CacheManager:
                 if page in self._ever_used[g]:
                     self.pages_reused += 1
                 self._ever_used[g].add(page)
-            if copies and group.tensors:
-                copy_pages(list(group.tensors.values()), [table[full]] * need, copies)
+            if copies:
+                for tensors in self._alike(group.tensors.values()):
+                    copy_pages(tensors, [table[full]] * need, copies)
         for tensors in self._alike(self.states.values()):
             if new_ids:
                 copy_pages(tensors, [parent.slot] * len(slots), slots)
@@ -355,8 +358,8 @@ class CacheManager:
             for table in group.tables.values():
                 table[:] = [moved.get(p, p) for p in table]
             self._ever_used[g].update(moved.values())
-            if group.tensors:
-                copy_pages(list(group.tensors.values()), list(moved), list(moved.values()))
+            for tensors in self._alike(group.tensors.values()):
+                copy_pages(tensors, list(moved), list(moved.values()))
         if total:
             for request in self._requests.values():
                 self._admissions += 1

@@ -220,11 +220,12 @@ class GenerationEngine:
 
     def abort(self, req_id: Hashable) -> Optional[Request]:
         """Take the request out wherever it is; its pages go back. What is still in flight for it is dropped."""
-        for first, waiting in self._forks.items():
+        for waiting in list(self._forks.values()):
             for request in waiting:
                 if request.req_id == req_id:
                     waiting.remove(request)
                     request.status, request.finish_reason = "finished", "abort"
+                    self._unfork(request)
                     return request
         request = self.scheduler.abort(req_id)
         if request is not None:

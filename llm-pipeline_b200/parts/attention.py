@@ -164,6 +164,8 @@ class PagedAttention(Mixer):
         if cache.pages is None or cache.group is None:
             raise RuntimeError("the attention mixer needs the pages of its cache")
         eight = cache.pages.dtype == torch.uint8
+        if eight and cache.page_size is None:
+            raise RuntimeError("pages in 8 bits do not show how many tokens they hold: the cache must say it (page_size)")
         page_size = cache.page_size if eight else cache.pages.shape[3]
         if self.tokens_per_tile is None:
             self.tokens_per_tile = kernels.tokens_per_attention_tile(self.num_heads, self.num_kv_heads, x.dtype,
@@ -247,7 +249,8 @@ class PagedAttention(Mixer):
 
     def attend_8bit(self, ctx, qkv: torch.Tensor, out: torch.Tensor, cache: LayerCache) -> None:
         """The same over pages in 8 bits: single tokens read them as they are (those at the front of a mixed step too: their pages
-        then need not be unpacked), for prompt portions the pages of their requests are unpacked first."""
+        then need not be unpacked), and so do prompt portions of few tokens over many; for the others the pages of their requests
+        are unpacked first (``ops.kv8``)."""
         tables = ctx.block_tables[cache.group]
         lead = ctx.num_requests if ctx.max_q_len == 1 else ctx.leading_single
         if lead:

@@ -149,6 +149,15 @@ def test_samples_that_find_no_room_are_computed_on_their_own(tmp_path):
     while core.has_unfinished():
         core.step()
     assert len(core._requests[others[0]].output) == 5 and core._requests[others[1]].status == "finished" and core.cache.num_live == 0
+    # one that waits for another that waits: the middle one goes, then the first
+    first = core.add_request(ids, 5, ignore_eos=True)
+    middle = core.add_request(ids, 5, ignore_eos=True, same_prompt_as=first)
+    last = core.add_request(ids, 5, ignore_eos=True, same_prompt_as=middle)
+    core.step()
+    core.abort(middle)
+    while core.has_unfinished():
+        core.step()
+    assert core._requests[first].output == core._requests[last].output and len(core._requests[last].output) == 5 and not core._forks
     with pytest.raises(ValueError, match="another prompt"):
         core.add_request(ids[:-1], 5, same_prompt_as=others[0])
 
