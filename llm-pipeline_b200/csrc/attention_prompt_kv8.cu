@@ -33,10 +33,11 @@
 #define P8_ROWS 128                                  // of a row tile
 #define P8_KEYS 128
 #define P8_THREADS 512
-#define P8_STAGES 2                                  // tiles of bytes on their way or being unpacked
+#define P8_STAGES 2                                  // tiles of bytes on their way or being unpacked, keys and values each
 #define P8_UNPACK 6                                  // warps that unpack
+#define P8_PIECES 3                                  // 16 bytes each that a lane unpacks side by side
 #define P8_HALF (P8_ROWS * 128)                      // bytes of 128 rows of 64 entries in half precision
-#define P8_RAW_STAGE (2 * P8_KEYS * P8_D)            // bytes of a tile's keys and values
+#define P8_RAW (P8_KEYS * P8_D)                      // bytes of a tile's keys, or values
 #define P8_SLOTS 8                                   // places for a tile's scales, which live until its softmax is done
 #define P8_PART (P8_D + 4)                           // floats of a row's sums: O, m, mu, l
 
@@ -55,11 +56,11 @@ struct Prompt8Params {
     int* error_flag;
 };
 
-__device__ __forceinline__ void p8_load_box(void* smem_dst, const CUtensorMap* map, int token, int kvh, int page, uint64_t* bar) {
+__device__ __forceinline__ void p8_load_box(void* smem_dst, const CUtensorMap* map, int token, int kvh, int kv, int page, uint64_t* bar) {
     const int zero = 0;
     asm volatile(
         "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n"
-        ::"r"(tc_smem_u32(smem_dst)), "l"(map), "r"(tc_smem_u32(bar)), "r"(zero), "r"(token), "r"(kvh), "r"(zero), "r"(page) : "memory");
+        ::"r"(tc_smem_u32(smem_dst)), "l"(map), "r"(tc_smem_u32(bar)), "r"(zero), "r"(token), "r"(kvh), "r"(kv), "r"(page) : "memory");
 }
 
 // Instruction descriptor of kind::f16 with half-precision operands and float32 sums, M x N.
@@ -74,6 +75,28 @@ __device__ __forceinline__ uint64_t p8_desc_mn(uint32_t smem_addr) {
 
 __device__ __forceinline__ void p8_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(tc_smem_u32(bar)) : "memory");
+}
+// One lane of a warp that executes this together: 1 there, 0 in the others.
+__device__ __forceinline__ uint32_t p8_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+    return one;
+}
+// Products and their commit by the thread whose `one` is not 0; the warp comes along. D[tmem] (+)= A[smem] B[smem]; A[tmem] B[smem].
+__device__ __forceinline__ void p8_mma(uint32_t one, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+                 ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void p8_mma_p(uint32_t one, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void p8_commit(uint32_t one, uint64_t* bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
+                 ::"r"(tc_smem_u32(bar)), "r"(one) : "memory");
 }
 __device__ __forceinline__ unsigned p8_half2(float lo, float hi) {
     unsigned r;
@@ -101,6 +124,9 @@ __device__ __forceinline__ float2 p8_add2(float2 a, float2 b) {
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
+
+// All ones in the bytes that are no number (0x7f and 0xff).
+__device__ __forceinline__ unsigned p8_no_number(unsigned w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu; }
 
 // Waits for this thread's tensor-memory loads. What they brought is named as changed by it: else the compiler may use the registers, which
 // it takes to be loaded where the load stands, before the wait.
@@ -159,31 +185,34 @@ template <int BOX>
 __global__ void __launch_bounds__(P8_THREADS, 1)
 prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p) {
     extern __shared__ unsigned char p8_raw[];
-    __shared__ __align__(8) uint64_t raw_full[P8_STAGES], raw_free[P8_STAGES], k_full, k_free, v_full[2], v_free[2], s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(8) uint64_t raw_full[2][P8_STAGES], raw_free[2][P8_STAGES], k_full[2], k_free[2], v_full, v_free, s_full[2], p_full[2], o_done[2];
     __shared__ __align__(16) float2 scales[P8_SLOTS][16];
     __shared__ unsigned no_number[P8_SLOTS][4];            // keys of a tile whose values hold NaN
     __shared__ uint32_t tmem_slot;
     const uint32_t raw_addr = tc_smem_u32(p8_raw);
     unsigned char* Qs = p8_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);     // [2 tiles][2 halves][128 rows][128 bytes]
-    unsigned char* Ks = Qs + 4 * P8_HALF;                        // [2 halves][128 keys][128 bytes]
-    unsigned char* Vs = Ks + 2 * P8_HALF;
-    unsigned char* raw = Vs + 4 * P8_HALF;                       // (two tiles of values before it) [P8_STAGES][box][keys, values][token][128 bytes]
+    unsigned char* Ks = Qs + 4 * P8_HALF;                        // [2 key tiles][2 halves][128 keys][128 bytes]
+    unsigned char* Vs = Ks + 4 * P8_HALF;                        // [2 halves][128 keys][128 bytes]
+    unsigned char* raw = Vs + 2 * P8_HALF;                       // [keys, values][P8_STAGES][128 keys][128 bytes]
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);      // (known to be one number for the warp: the roles do not diverge)
     if (warp == 8 && lane == 0) {
         for (int i = 0; i < P8_STAGES; ++i) {
-            mbar_init(&raw_full[i], 2);                          // the boxes, and the scales
-            mbar_init(&raw_free[i], P8_UNPACK);
+            mbar_init(&raw_full[0][i], 2);                       // the boxes, and the scales
+            mbar_init(&raw_full[1][i], 1);
+            mbar_init(&raw_free[0][i], P8_UNPACK);
+            mbar_init(&raw_free[1][i], P8_UNPACK);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&v_full[i], P8_UNPACK);
-            mbar_init(&v_free[i], 1);
+            mbar_init(&k_full[i], P8_UNPACK);
+            mbar_init(&k_free[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
         }
-        mbar_init(&k_full, P8_UNPACK);
-        mbar_init(&k_free, 1);
+        mbar_init(&v_full, P8_UNPACK);
+        mbar_init(&v_free, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
     }
@@ -260,47 +289,47 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
     const uint32_t tmem = tmem_slot;                             // S of the tiles in columns 0 and 128, O in 256 and 384
 
     if (warp == 15) {
-        // ---- products ----
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = p8_idesc(P8_ROWS, P8_KEYS), idesc_o = p8_idesc(P8_ROWS, P8_D) | (1u << 16);      // V is MN-major
-            // (an operand further on in shared memory: its address in units of 16 bytes, in the descriptor's low bits)
-            const uint64_t q_desc = umma_desc(tc_smem_u32(Qs)), k_desc = umma_desc(tc_smem_u32(Ks)), v_desc = p8_desc_mn(tc_smem_u32(Vs));
-            const int last_t = n[1] > 0 ? 1 : 0;
-            // S of row tile t and key tile j; the first of the row tiles waits for the keys, the last frees them
-            auto scores = [&](int t, int j) {
-                if (t == 0 || j >= n[0]) mbar_wait(&k_full, j & 1, p.error_flag);
-                // S lies where the P of the key tile before is: products into other columns keep no order among themselves
-                if (j > 0) mbar_wait(&o_done[t], (j - 1) & 1, p.error_flag);
+        // ---- products: the whole warp walks along, one thread issues (addresses then stay in uniform registers: with the
+        // loop in one thread's branch eight products took 450 to 950 clocks to issue, a third of a key tile's time) ----
+        constexpr uint32_t idesc_s = p8_idesc(P8_ROWS, P8_KEYS), idesc_o = p8_idesc(P8_ROWS, P8_D) | (1u << 16);      // V is MN-major
+        const uint32_t one = p8_elect();
+        // (an operand further on in shared memory: its address in units of 16 bytes, in the descriptor's low bits)
+        const uint64_t q_desc = umma_desc(tc_smem_u32(Qs)), k_desc = umma_desc(tc_smem_u32(Ks)), v_desc = p8_desc_mn(tc_smem_u32(Vs));
+        const int last_t = n[1] > 0 ? 1 : 0;
+        // S of row tile t and key tile j; the first of the row tiles waits for the keys, the last frees them
+        auto scores = [&](int t, int j) {
+            if (t == 0 || j >= n[0]) mbar_wait(&k_full[j & 1], (j >> 1) & 1, p.error_flag);
+            // S lies where the P of the key tile before is: products into other columns keep no order among themselves
+            if (j > 0) mbar_wait(&o_done[t], (j - 1) & 1, p.error_flag);
+            fa_fence_after();
+            const uint64_t q_at = q_desc + (uint32_t)t * (2 * P8_HALF >> 4), k_at = k_desc + (uint32_t)(j & 1) * (2 * P8_HALF >> 4);
+#pragma unroll
+            for (int k = 0; k < P8_D / 16; ++k) {
+                const uint32_t off = ((uint32_t)(k >> 2) * P8_HALF + (uint32_t)(k & 3) * 32) >> 4;
+                p8_mma(one, tmem + t * 128, q_at + off, k_at + off, idesc_s, k != 0 ? 1u : 0u);
+            }
+            p8_commit(one, &s_full[t]);
+            if (t == last_t || (t == 0 && j >= n[1])) p8_commit(one, &k_free[j & 1]);
+        };
+#pragma unroll 1
+        for (int j = -1; j < tiles; ++j) {
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                const int count = t == 0 ? n[0] : n[1];
+                if (j >= count) continue;
+                if (j < 0) {
+                    if (count > 0) scores(t, 0);
+                    continue;
+                }
+                mbar_wait(&p_full[t], j & 1, p.error_flag);
+                if (t == 0 || j >= n[0]) mbar_wait(&v_full, j & 1, p.error_flag);
                 fa_fence_after();
-                const uint64_t q_at = q_desc + (uint32_t)t * (2 * P8_HALF >> 4);
 #pragma unroll
-                for (int k = 0; k < P8_D / 16; ++k) {
-                    const uint32_t off = ((uint32_t)(k >> 2) * P8_HALF + (uint32_t)(k & 3) * 32) >> 4;
-                    umma_f16(tmem + t * 128, q_at + off, k_desc + off, idesc_s, k != 0 ? 1u : 0u);
-                }
-                umma_commit(&s_full[t]);
-                if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&k_free);
-            };
-#pragma unroll 1
-            for (int j = -1; j < tiles; ++j) {
-#pragma unroll 1
-                for (int t = 0; t < 2; ++t) {
-                    const int count = t == 0 ? n[0] : n[1];
-                    if (j >= count) continue;
-                    if (j < 0) {
-                        if (count > 0) scores(t, 0);
-                        continue;
-                    }
-                    mbar_wait(&p_full[t], j & 1, p.error_flag);
-                    if (t == 0 || j >= n[0]) mbar_wait(&v_full[j & 1], (j >> 1) & 1, p.error_flag);
-                    fa_fence_after();
-#pragma unroll
-                    for (int k = 0; k < P8_KEYS / 16; ++k)       // 16 keys a product: 8 columns of P, 2 KB of V
-                        fa_umma_a_tmem(tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc + (uint32_t)(((j & 1) * 2 * P8_HALF + k * 2048) >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
-                    umma_commit(&o_done[t]);
-                    if (t == last_t || (t == 0 && j >= n[1])) umma_commit(&v_free[j & 1]);
-                    if (j + 1 < count) scores(t, j + 1);
-                }
+                for (int k = 0; k < P8_KEYS / 16; ++k)           // 16 keys a product: 8 columns of P, 2 KB of V
+                    p8_mma_p(one, tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc + (uint32_t)(k * 2048 >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
+                p8_commit(one, &o_done[t]);
+                if (t == last_t || (t == 0 && j >= n[1])) p8_commit(one, &v_free);
+                if (j + 1 < count) scores(t, j + 1);
             }
         }
     } else if (warp == 14) {
@@ -320,72 +349,114 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
                 ev = at[p.nkv];
             }
         };
-        int now = find(0), next = find(1);
+        // one tile's keys or values; out of range: the box arrives as zeros
+        auto load = [&](int kv, int j, int page) {
+            const int stage = j % P8_STAGES;
+            if (j >= P8_STAGES) mbar_wait(&raw_free[kv][stage], (j / P8_STAGES - 1) & 1, p.error_flag);
+            if (lane == 0) mbar_expect_tx(&raw_full[kv][stage], P8_RAW);
+            __syncwarp();
+            if (boxes)
+                p8_load_box(raw + (kv * P8_STAGES + stage) * P8_RAW + lane * 8 * P8_D, &map, ((t_begin + j) * P8_KEYS + lane * 8) & (p.page_size - 1), kvh, kv,
+                            page >= 0 ? page : p.num_pages, &raw_full[kv][stage]);
+        };
+        int now = find(0), next = find(1), before = -1;
         ask(now);
-        for (int j = 0; j < tiles; ++j) {
-            const int after = find(j + 2), stage = j % P8_STAGES;
-            if (j >= P8_STAGES) mbar_wait(&raw_free[stage], (j / P8_STAGES - 1) & 1, p.error_flag);
-            if (lane == 0) mbar_expect_tx(&raw_full[stage], P8_RAW_STAGE);
-            __syncwarp();
-            if (boxes)                                           // out of range: the box arrives as zeros
-                p8_load_box(raw + stage * P8_RAW_STAGE + lane * 8 * 2 * P8_D, &map, ((t_begin + j) * P8_KEYS + lane * 8) & (p.page_size - 1), kvh,
-                            now >= 0 ? now : p.num_pages, &raw_full[stage]);
-            if (lane < 16)                                       // (a block of zeros may have any scale; the operands are 2^-8 of the bytes' values)
-                scales[j % P8_SLOTS][lane] = now >= 0 ? make_float2((ek == 0u ? 1.f : kv8_scale(ek)) * 256.f, (float)((int)ev - 119)) : make_float2(1.f, -INFINITY);
-            if (lane < 4) no_number[j % P8_SLOTS][lane] = 0u;
-            __syncwarp();
-            if (lane == 0) p8_arrive(&raw_full[stage]);
-            now = next;
-            next = after;
-            ask(now);
+#pragma unroll 1
+        for (int j = 0; tiles > 0 && j <= tiles; ++j) {          // in the order in which they are unpacked: keys a tile ahead of values
+            if (j < tiles) {
+                const int after = find(j + 2);
+                load(0, j, now);
+                if (lane < 16)                                   // (a block of zeros may have any scale; the operands are 2^-8 of the bytes' values)
+                    scales[j % P8_SLOTS][lane] = now >= 0 ? make_float2((ek == 0u ? 1.f : kv8_scale(ek)) * 256.f, (float)((int)ev - 119)) : make_float2(1.f, -INFINITY);
+                if (lane < 4) no_number[j % P8_SLOTS][lane] = 0u;
+                __syncwarp();
+                if (lane == 0) p8_arrive(&raw_full[0][j % P8_STAGES]);
+                if (j > 0) load(1, j - 1, before);
+                before = now;
+                now = next;
+                next = after;
+                ask(now);
+            } else {
+                load(1, j - 1, before);
+            }
         }
     } else if (warp >= 8) {
         // ---- unpacking ----
         // Eight lanes take a key: lane c of them its entries 16 c .. 16 c + 15.
         const int first = tid - 256, piece = first & 7, half = piece >> 2, at = (piece & 3) * 2;
-        for (int j = 0; j < tiles; ++j) {
-            const unsigned char* src = raw + j % P8_STAGES * P8_RAW_STAGE;
+        // Keys are unpacked a tile ahead of values: K 0, K 1, V 0, K 2, V 1 .. : a tile's keys then wait for nobody, and its
+        // values are due only when its softmax is done.
+#pragma unroll 1
+        for (int step = 0; step <= 2 * tiles; ++step) {
+            const int kv = step > 0 && (step & 1) == 0, j = kv ? step / 2 - 1 : (step + 1) / 2;
+            if (j == tiles) continue;
+            const unsigned char* src = raw + (kv * P8_STAGES + j % P8_STAGES) * P8_RAW;
             const float2* of = scales[j % P8_SLOTS];
-            mbar_wait(&raw_full[j % P8_STAGES], j / P8_STAGES & 1, p.error_flag);
+            mbar_wait(&raw_full[kv][j % P8_STAGES], j / P8_STAGES & 1, p.error_flag);
             const int there = ctx - (t_begin + j) * P8_KEYS;     // keys of the tile that exist
             const bool whole = there >= P8_KEYS && __all_sync(0xffffffffu, of[lane & 15].y > -INFINITY);
+            if (kv == 0 && j > 1) mbar_wait(&k_free[j & 1], ((j >> 1) - 1) & 1, p.error_flag);
+            if (kv == 1 && j > 0) mbar_wait(&v_free, (j - 1) & 1, p.error_flag);
+            unsigned char* dst = (kv == 0 ? Ks + (j & 1) * 2 * P8_HALF : Vs) + half * P8_HALF;
 #pragma unroll 1
-            for (int kv = 0; kv < 2; ++kv) {
-                if (kv == 0 && j > 0) mbar_wait(&k_free, (j - 1) & 1, p.error_flag);
-                if (kv == 1 && j > 1) mbar_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, p.error_flag);
-                unsigned char* dst = (kv == 0 ? Ks : Vs + (j & 1) * 2 * P8_HALF) + half * P8_HALF;
-#pragma unroll 2
-                for (int key = first >> 3; key < P8_KEYS; key += P8_UNPACK * 4) {
-                    const uint4 four = *reinterpret_cast<const uint4*>(src + ((key / BOX) * 2 + kv) * BOX * P8_D + (key % BOX) * P8_D + ((piece ^ (key & 7)) << 4));
-                    unsigned w[4] = {four.x, four.y, four.z, four.w};
-                    if (!whole && (key >= there || of[key / 8].y == -INFINITY)) w[0] = w[1] = w[2] = w[3] = 0u;      // not there: zeros, for factors of zero
-                    unsigned any = 0u, h[8];
+            for (int key0 = first >> 3; key0 < P8_KEYS; key0 += P8_PIECES * P8_UNPACK * 4) {
+                uint4 w[P8_PIECES];
+                unsigned any = 0u;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        any |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;
-                        // a byte seeeemmm is s0eeeemmm0000000 in half precision, times 2^8; of four bytes the pairs 0, 2 and 1, 3
-                        h[2 * i] = ((w[i] << 7) & 0x3f803f80u) | ((w[i] << 8) & 0x80008000u);
-                        h[2 * i + 1] = ((w[i] >> 1) & 0x3f803f80u) | (w[i] & 0x80008000u);
+                for (int u = 0; u < P8_PIECES; ++u) {
+                    const int key = key0 + u * P8_UNPACK * 4;
+                    w[u] = make_uint4(0u, 0u, 0u, 0u);
+                    if (key < P8_KEYS) w[u] = *reinterpret_cast<const uint4*>(src + key * P8_D + ((piece ^ (key & 7)) << 4));
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int u = 0; u < P8_PIECES; ++u) {        // not there: zeros, for factors of zero
+                        const int key = key0 + u * P8_UNPACK * 4;
+                        if (key >= there || of[min(key, P8_KEYS - 1) / 8].y == -INFINITY) w[u] = make_uint4(0u, 0u, 0u, 0u);
                     }
-                    if (__builtin_expect(any & 0x80808080u, 0)) {        // what is no number: zeros as values, and the key is noted
+                }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            w[i] &= ~(((((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
-                            h[2 * i] = ((w[i] << 7) & 0x3f803f80u) | ((w[i] << 8) & 0x80008000u);
-                            h[2 * i + 1] = ((w[i] >> 1) & 0x3f803f80u) | (w[i] & 0x80008000u);
-                        }
+                for (int u = 0; u < P8_PIECES; ++u)
+                    any |= ((w[u].x & 0x7f7f7f7fu) + 0x01010101u) | ((w[u].y & 0x7f7f7f7fu) + 0x01010101u) | ((w[u].z & 0x7f7f7f7fu) + 0x01010101u) |
+                           ((w[u].w & 0x7f7f7f7fu) + 0x01010101u);
+                if (__builtin_expect(any & 0x80808080u, 0)) {            // what is no number: zeros as values, and the key is noted
+#pragma unroll 1
+                    for (int u = 0; u < P8_PIECES; ++u) {
+                        const int key = key0 + u * P8_UNPACK * 4;
+                        uint4 x = u == 0 ? w[0] : u == 1 ? w[1] : w[2];
+                        const unsigned bad[4] = {p8_no_number(x.x), p8_no_number(x.y), p8_no_number(x.z), p8_no_number(x.w)};
+                        if ((bad[0] | bad[1] | bad[2] | bad[3]) == 0u) continue;
+                        x = make_uint4(x.x & ~bad[0], x.y & ~bad[1], x.z & ~bad[2], x.w & ~bad[3]);
+                        if (u == 0) w[0] = x;
+                        if (u == 1) w[1] = x;
+                        if (u == 2) w[2] = x;
                         atomicOr(&no_number[j % P8_SLOTS][key >> 5], 1u << (key & 31));
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < P8_PIECES; ++u) {
+                    const int key = key0 + u * P8_UNPACK * 4;
+                    const unsigned b[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+                    unsigned h[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {                // a byte seeeemmm is s0eeeemmm0000000 in half precision, times 2^8; of four bytes the pairs 0, 2 and 1, 3
+                        h[2 * i] = ((b[i] << 7) & 0x3f803f80u) | ((b[i] << 8) & 0x80008000u);
+                        h[2 * i + 1] = ((b[i] >> 1) & 0x3f803f80u) | (b[i] & 0x80008000u);
                     }
                     // (lanes of the second half of the head store their second piece first: the halves lie in the same banks)
                     const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-                    *reinterpret_cast<uint4*>(dst + key * 128 + (((at + half) ^ (key & 7)) << 4)) = half ? hi : lo;
-                    *reinterpret_cast<uint4*>(dst + key * 128 + (((at + 1 - half) ^ (key & 7)) << 4)) = half ? lo : hi;
+                    if (key < P8_KEYS) {
+                        *reinterpret_cast<uint4*>(dst + key * 128 + (((at + half) ^ (key & 7)) << 4)) = half ? hi : lo;
+                        *reinterpret_cast<uint4*>(dst + key * 128 + (((at + 1 - half) ^ (key & 7)) << 4)) = half ? lo : hi;
+                    }
                 }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                __syncwarp();
-                if (lane == 0) p8_arrive(kv == 0 ? &k_full : &v_full[j & 1]);
             }
-            if (lane == 0) p8_arrive(&raw_free[j % P8_STAGES]);
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                p8_arrive(kv == 0 ? &k_full[j & 1] : &v_full);
+                p8_arrive(&raw_free[kv][j % P8_STAGES]);
+            }
         }
     } else {
         // ---- softmax ----
@@ -606,12 +677,12 @@ LLMP_API int llmp_kv8_prompt(const void* q, long q_stride, void* out, long out_s
     const cuuint64_t row = P8_D, plane = row * page_size;
     const cuuint64_t dims[5] = {P8_D, (cuuint64_t)page_size, (cuuint64_t)nkv, 2, (cuuint64_t)num_pages};
     const cuuint64_t strides[4] = {row, plane, plane * nkv, (cuuint64_t)p.page_bytes};
-    const cuuint32_t box[5] = {P8_D, (cuuint32_t)box_tokens, 1, 2, 1};
+    const cuuint32_t box[5] = {P8_D, (cuuint32_t)box_tokens, 1, 1, 1};
     const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
     const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     LLMP_REQUIRE(rc == CUDA_SUCCESS, "kv8 prompt attention: cuTensorMapEncodeTiled failed with code %d", (int)rc);
-    const size_t smem = 10 * (size_t)P8_HALF + P8_STAGES * (size_t)P8_RAW_STAGE + 1024;
+    const size_t smem = 10 * (size_t)P8_HALF + 2 * P8_STAGES * (size_t)P8_RAW + 1024;
     const auto kernel = box_tokens == 8 ? prompt_kv8_kernel<8> : box_tokens == 16 ? prompt_kv8_kernel<16> : prompt_kv8_kernel<32>;
     if (box_tokens == 8) LLMP_ALLOW_SMEM(prompt_kv8_kernel<8>, smem);
     else if (box_tokens == 16) LLMP_ALLOW_SMEM(prompt_kv8_kernel<16>, smem);
