@@ -6,10 +6,14 @@
 //   unpack       six warps turn a tile's bytes into half precision, laid out as operands; both row tiles use what is unpacked once. By
 //                shifts and masks: the conversion instruction is as slow as the exponentials and shares their unit
 //   S = Q K^T    Q, K in shared memory (128-byte swizzle, K-major), S in tensor memory
-//   softmax      a thread has a row: it reads S from tensor memory twice (maxima; factors), 32 columns at a time in loops that stay
-//                short (unrolled whole, the instructions do not come fast enough: 112 us for 2,048 tokens), and writes factors over S
+//   softmax      a thread has a row: it reads S from tensor memory twice (maxima; factors), 32 columns at a time, and writes factors
+//                over S. The loops stay short and what is rare stands outside them (masks, weights that factors do not give, values that
+//                are no number), since the instructions of four roles do not come fast enough otherwise: 2,048 tokens behind 14,000
+//                took 771 us with 64 columns a turn and all of it inside, 741 with 32, 661 so; one pass, with the rescaling inside, 846
 //   O += P V     P read from tensor memory, V in shared memory MN-major, O in tensor memory
 // While one row tile is in its softmax the tensor cores work for the other. The two tiles' S and O fill the tensor memory (512 columns).
+// What bounds it: a row tile's chain of S, maxima, factors, P V, one after another, 5,000 clocks a key tile, of them the softmax 3,100 and
+// the products 1,030. 2,048 tokens (32 heads) 66.6 us, 0.52 PFLOP/s; behind 14,000 657 us, 0.77 PFLOP/s; 40 behind 8,000 30.9 us.
 //
 // With t = log2(e) scale q.k and a value's scale 2^v, weights are 2^t and the factor of a value's bytes is 2^(t + v). As in
 // attention_decode_kv8_stream.cu each has its own maximum, m and mu, raised to a whole number when it is passed by more than 12: factors
@@ -141,7 +145,7 @@ __device__ __forceinline__ void p8_wait_ld(uint32_t (&r)[32]) {
 
 // The largest t and t + v of 32 scores (hidden ones are -inf). `scales`: of the 32 / BLOCK blocks they belong to, every BLOCK / 8th: the
 // keys' scale, the exponent of the values' (-inf: a page that is missing).
-template <int BLOCK> __device__ __forceinline__ void p8_top(const uint32_t (&x)[32], const float2* scales, float f, float& t_top, float& u_top) {
+template <int BLOCK> __device__ __forceinline__ void p8_top(const uint32_t (&x)[32], const float2* scales, float f, float& t_top, float& u_top, float& v_low) {
 #pragma unroll
     for (int b = 0; b < 32; b += BLOCK) {
         const float2 s = scales[b / 8];
@@ -151,6 +155,7 @@ template <int BLOCK> __device__ __forceinline__ void p8_top(const uint32_t (&x)[
         const float t = s.y == -INFINITY ? -INFINITY : top * fmaxf(s.x * f, 1e-38f);
         t_top = fmaxf(t_top, t);
         u_top = fmaxf(u_top, t + s.y);
+        v_low = fminf(v_low, s.y == -INFINITY ? INFINITY : s.y);
     }
 }
 
@@ -170,10 +175,20 @@ __device__ __forceinline__ float p8_factors(const uint32_t (&x)[32], const float
             sum = i == 0 ? v : p8_add2(sum, v);
             pk[(b + i) / 2] = p8_half2(v.x, v.y);
         }
-        const float n = mu - m - s.y;                            // weight = factor * 2^n
-        if (__builtin_expect(n <= 100.f, 1)) {
-            l = fmaf(sum.x + sum.y, p8_power(fmaxf(n, -126.f)), l);
-        } else if (s.y > -INFINITY) {                            // factors too small for float32 although their weights are not
+        const float n = mu - m - s.y;                            // weight = factor * 2^n; beyond 2^100 they are p8_far's
+        l = fmaf(sum.x + sum.y, n <= 100.f ? p8_power(fmaxf(n, -126.f)) : 0.f, l);
+    }
+    return l;
+}
+
+// The sum of the weights that p8_factors leaves out: factors too small for float32 although their weights are not.
+template <int BLOCK> __device__ __forceinline__ float p8_far(const uint32_t (&x)[32], const float2* scales, float f, float m, float mu) {
+    float l = 0.f;
+#pragma unroll
+    for (int b = 0; b < 32; b += BLOCK) {
+        const float2 s = scales[b / 8];
+        if (mu - m - s.y > 100.f && s.y > -INFINITY) {
+            const float c = fmaxf(s.x * f, 1e-38f);
 #pragma unroll
             for (int i = 0; i < BLOCK; ++i) l += fa_ex2(fmaf(__uint_as_float(x[b + i]), c, -m));
         }
@@ -185,9 +200,9 @@ template <int BOX>
 __global__ void __launch_bounds__(P8_THREADS, 1)
 prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p) {
     extern __shared__ unsigned char p8_raw[];
-    __shared__ __align__(8) uint64_t raw_full[2][P8_STAGES], raw_free[2][P8_STAGES], k_full[2], k_free[2], v_full, v_free, s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(8) uint64_t raw_full[2][P8_STAGES], raw_free[2][P8_STAGES], k_full[2], k_free[2], v_full, v_free, s_full[2], p_full[2][2], o_done[2];
     __shared__ __align__(16) float2 scales[P8_SLOTS][16];
-    __shared__ unsigned no_number[P8_SLOTS][4];            // keys of a tile whose values hold NaN
+    __shared__ __align__(16) unsigned no_number[P8_SLOTS][4];            // keys of a tile whose values hold NaN
     __shared__ uint32_t tmem_slot;
     const uint32_t raw_addr = tc_smem_u32(p8_raw);
     unsigned char* Qs = p8_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);     // [2 tiles][2 halves][128 rows][128 bytes]
@@ -208,7 +223,8 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
             mbar_init(&k_full[i], P8_UNPACK);
             mbar_init(&k_free[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i][0], 4);
+            mbar_init(&p_full[i][1], 4);
             mbar_init(&o_done[i], 1);
         }
         mbar_init(&v_full, P8_UNPACK);
@@ -321,12 +337,15 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
                     if (count > 0) scores(t, 0);
                     continue;
                 }
-                mbar_wait(&p_full[t], j & 1, p.error_flag);
                 if (t == 0 || j >= n[0]) mbar_wait(&v_full, j & 1, p.error_flag);
-                fa_fence_after();
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    mbar_wait(&p_full[t][half], j & 1, p.error_flag);
+                    fa_fence_after();
 #pragma unroll
-                for (int k = 0; k < P8_KEYS / 16; ++k)           // 16 keys a product: 8 columns of P, 2 KB of V
-                    p8_mma_p(one, tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc + (uint32_t)(k * 2048 >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
+                    for (int k = 0; k < P8_KEYS / 32; ++k)       // 16 keys a product: 8 columns of P, 2 KB of V
+                        p8_mma_p(one, tmem + 256 + t * 128, tmem + t * 128 + half * 32 + k * 8, v_desc + (uint32_t)((half * 4 + k) * 2048 >> 4), idesc_o, (j | half | k) != 0 ? 1u : 0u);
+                }
                 p8_commit(one, &o_done[t]);
                 if (t == last_t || (t == 0 && j >= n[1])) p8_commit(one, &v_free);
                 if (j + 1 < count) scores(t, j + 1);
@@ -470,7 +489,7 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         const int pos_first = pos0 + tok0 + mine * P8_ROWS / G, pos_last = pos0 + tok0 + (min(rows, (mine + 1) * P8_ROWS) - 1) / G;
         float m = -INFINITY, mu = -INFINITY, l = 0.f;
         const int count = n[mine];
-        uint32_t x[32], y[32], pk[16];
+        uint32_t x[32], pk[16];
         constexpr int BLOCK = BOX;
         for (int j = 0; j < count; ++j) {
             const int j0 = (t_begin + j) * P8_KEYS;
@@ -478,17 +497,22 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
             const bool mask = j0 + P8_KEYS - 1 > pos_first || (p.window > 0 && j0 < pos_last - p.window + 1) || rows < (mine + 1) * P8_ROWS;
             mbar_wait(&s_full[mine], j & 1, p.error_flag);       // P V of the key tile before is done as well: it was issued before
             fa_fence_after();
-            float t_top = -INFINITY, u_top = -INFINITY;
+            if (mask) {                                          // what is hidden is written over S, once
 #pragma unroll 1
-            for (int c = 0; c < P8_KEYS; c += 64) {
+                for (int c = 0; c < P8_KEYS; c += 32) {
+                    FA_TMEM_LD32(ts + c, x, 0);
+                    p8_wait_ld(x);
+                    fa_mask32(x, j0 + c, pos, first);
+                    FA_TMEM_ST32(ts + c, x, 0);
+                }
+                fa_tmem_wait_st();
+            }
+            float t_top = -INFINITY, u_top = -INFINITY, v_low = INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < P8_KEYS; c += 32) {
                 FA_TMEM_LD32(ts + c, x, 0);
                 p8_wait_ld(x);
-                FA_TMEM_LD32(ts + c + 32, y, 0);
-                if (mask) fa_mask32(x, j0 + c, pos, first);
-                p8_top<BLOCK>(x, of + c / 8, f, t_top, u_top);
-                p8_wait_ld(y);
-                if (mask) fa_mask32(y, j0 + c + 32, pos, first);
-                p8_top<BLOCK>(y, of + c / 8 + 4, f, t_top, u_top);
+                p8_top<BLOCK>(x, of + c / 8, f, t_top, u_top, v_low);
             }
             if (t_top > m + 12.f) {
                 const float to_m = ceilf(t_top);
@@ -513,33 +537,35 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
                 }
             }
             const float m_now = m == -INFINITY ? 0.f : m, mu_now = mu == -INFINITY ? 0.f : mu;
-            // factors over the first 64 columns of S, always over columns that were read before
+            if (__any_sync(0xffffffffu, mu_now - m_now - v_low > 100.f)) {
 #pragma unroll 1
-            for (int c = 0; c < P8_KEYS; c += 64) {
+                for (int c = 0; c < P8_KEYS; c += 32) {
+                    FA_TMEM_LD32(ts + c, x, 0);
+                    p8_wait_ld(x);
+                    l += p8_far<BLOCK>(x, of + c / 8, f, m_now, mu_now);
+                }
+            }
+#pragma unroll 1
+            for (int c = 0; c < P8_KEYS; c += 32) {
                 FA_TMEM_LD32(ts + c, x, 0);
                 p8_wait_ld(x);
-                FA_TMEM_LD32(ts + c + 32, y, 0);
-                if (mask) fa_mask32(x, j0 + c, pos, first);
                 l += p8_factors<BLOCK>(x, of + c / 8, f, m_now, mu_now, pk);
-                p8_wait_ld(y);
                 FA_TMEM_ST16(ts + c / 2, pk);
-                if (mask) fa_mask32(y, j0 + c + 32, pos, first);
-                l += p8_factors<BLOCK>(y, of + c / 8 + 4, f, m_now, mu_now, pk);
-                FA_TMEM_ST16(ts + c / 2 + 16, pk);
+                if (c & 32) {                                    // half of the keys: their product may begin (661 -> 657 us)
+                    fa_tmem_wait_st();
+                    fa_fence_before();
+                    __syncwarp();
+                    if (lane == 0) p8_arrive(&p_full[mine][c >> 6]);
+                }
             }
-            fa_tmem_wait_st();
-            fa_fence_before();
-            __syncwarp();
-            if (lane == 0) p8_arrive(&p_full[mine]);
             // values that are no number: looked at once the tile's values are unpacked, which the next wait stands behind
             if (j > 0) {
                 const int before = (j - 1) % P8_SLOTS, k0 = j0 - P8_KEYS;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const unsigned bad = no_number[before][w];
-                    if (bad != 0u)
-                        for (int i = 0; i < 32; ++i)
-                            if ((bad >> i & 1u) && k0 + w * 32 + i >= first && k0 + w * 32 + i <= pos) l = __int_as_float(0x7fffffff);
+                const uint4 bad = *reinterpret_cast<const uint4*>(no_number[before]);
+                if (__builtin_expect((bad.x | bad.y | bad.z | bad.w) != 0u, 0)) {
+#pragma unroll 1
+                    for (int i = 0; i < P8_KEYS; ++i)
+                        if ((no_number[before][i >> 5] >> (i & 31) & 1u) && k0 + i >= first && k0 + i <= pos) l = __int_as_float(0x7fffffff);
                 }
             }
         }
@@ -547,12 +573,11 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         fa_fence_after();
         if (count > 0) {
             const int before = (count - 1) % P8_SLOTS, k0 = (t_begin + count - 1) * P8_KEYS;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const unsigned bad = no_number[before][w];
-                if (bad != 0u)
-                    for (int i = 0; i < 32; ++i)
-                        if ((bad >> i & 1u) && k0 + w * 32 + i >= first && k0 + w * 32 + i <= pos) l = __int_as_float(0x7fffffff);
+            const uint4 bad = *reinterpret_cast<const uint4*>(no_number[before]);
+            if ((bad.x | bad.y | bad.z | bad.w) != 0u) {
+#pragma unroll 1
+                for (int i = 0; i < P8_KEYS; ++i)
+                    if ((no_number[before][i >> 5] >> (i & 31) & 1u) && k0 + i >= first && k0 + i <= pos) l = __int_as_float(0x7fffffff);
             }
         }
         const float inv = l == 0.f ? 0.f : exp2f(mu - m) / l;    // no keys: zeros

@@ -1,9 +1,11 @@
 """Attention of prompt portions over pages of 8-bit keys and values (``cache.spec.KV8PagesSpec``).
 
-Few bfloat16 queries of head size 128 over many keys go to a kernel that reads the pages as they are
-(``kernels.kv8_prompt_attention``; ``reads_pages_directly`` says when). For all others the pages that a step's portions see are unpacked into a workspace of the query's type, laid out as ordinary
-pages, and the attention kernels of ordinary pages run over it (``kernels.paged_attention``): a page's values are exact in
-either type (the scales are powers of two), so the result is exactly what they give for a cache that holds these values."""
+bfloat16 queries of head size 128 go to a kernel that reads the pages as they are (``kernels.kv8_prompt_attention``) where that is
+faster: few queries over many keys above all (``reads_pages_directly``). For all others the pages that a step's portions see are
+unpacked into a workspace of the query's type, laid out as ordinary pages, and the attention kernels of ordinary pages run over it
+(``kernels.paged_attention``): a page's values are exact in either type (the scales are powers of two), so the result is exactly what
+they give for a cache that holds these values. A value that is no number makes the whole rows of a head that see it no numbers in the
+one kernel, their entry of the value's column in the others."""
 
 from __future__ import annotations
 
@@ -64,23 +66,27 @@ def reads_pages_directly(starts: Sequence[int], q_lens: Sequence[int], first_req
     """Whether a step's portions are better served by the kernel that reads 8-bit pages (256 query rows an item, its bytes unpacked in
     every one) than by unpacking the pages once and the attention kernel of ordinary pages (128 rows, two of them on an SM; keys
     shared by at most 8 items of at least 16 tiles). By what each takes, in us on a B200 (head size 128, 8 key/value heads):
-    18 and 4.5 a key tile of the longest part, against 8, 1.9 for every 1,000 tokens of the pages, and the longer of 2.8 a key tile
-    of the longest item and 2.2 for every key tile an SM has. Measured (direct, unpacked), 32 query heads: 40 new tokens behind 8,000
-    37, 70; 128 behind 2,000 33, 48; 256 behind 8,000 86, 85; 64 behind 500 26, 22; 2,048 new ones 86, 71; 2,048 behind 14,000 922, 604."""
+    18 and the longer of 2.75 a key tile of the longest part and 3.2 for every key tile an SM has, against 8, 1.9 for every 1,000 tokens of
+    the pages, and the longer of 2.8 a key tile of the longest item and 1.3 for every key tile an SM has, with up to 18 for the end. Measured
+    (direct, unpacked), 32 query heads: 40 new tokens behind 8,000 31, 71; 128 behind 2,000 29, 48; 512 behind 8,000 113, 131; 1,024 behind
+    8,000 206, 209; 2,048 new ones 66, 70; 64 behind 500 24, 22; 1,000 new ones 35, 31; 4,000 new ones 200, 181; 2,048 behind 14,000 657, 606."""
     group = num_heads // num_kv_heads
     wide = tiles_of(starts, q_lens, first_request, max(1, 256 // group), window)
-    if not wide or len(wide) * num_kv_heads > sms:
+    if not wide:
         return False
     longest, places = 0, plan_items(starts, q_lens, first_request, max(1, 256 // group), num_kv_heads, window, sms, 1 << 30)[1]
     cut = {(r, t): k for r, t, k, _p in places}
     for n, r, t in wide:
         longest = max(longest, -(-n // cut.get((r, t), 1)))
+    direct = 2.75 * longest
+    if len(wide) * num_kv_heads > sms:
+        direct = max(direct, 3.2 * sum(n for n, _r, _t in wide) * num_kv_heads / sms)
     narrow = tiles_of(starts, q_lens, first_request, max(1, 128 // group), window)
     blocks, most = len(narrow) * num_kv_heads, max(n for n, _r, _t in narrow)
     segments = min(8, 4 * sms // blocks, most // 16) if blocks <= sms else 1
     tokens = sum(s + n - (max(0, s - window + 1) if window else 0) for s, n in zip(starts[first_request:], q_lens[first_request:]) if n)
-    unpacked = 8 + 1.9e-3 * tokens * num_kv_heads / 8 + max(2.8 * -(-most // max(1, segments)), 2.2 * sum(n for n, _r, _t in narrow) * num_kv_heads / sms)
-    return 18 + 4.5 * longest < unpacked
+    unpacked = max(2.8 * -(-most // max(1, segments)), 1.3 * sum(n for n, _r, _t in narrow) * num_kv_heads / sms + min(1.1 * most, 18))
+    return 18 + direct < 8 + 1.9e-3 * tokens * num_kv_heads / 8 + unpacked
 
 
 class PromptPlan:

@@ -249,7 +249,7 @@ class PagedAttention(Mixer):
 
     def attend_8bit(self, ctx, qkv: torch.Tensor, out: torch.Tensor, cache: LayerCache) -> None:
         """The same over pages in 8 bits: single tokens read them as they are (those at the front of a mixed step too: their pages
-        then need not be unpacked), and so do prompt portions of few tokens over many; for the others the pages of their requests
+        then need not be unpacked), and so do prompt portions where that is faster; for the others the pages of their requests
         are unpacked first (``ops.kv8``)."""
         tables = ctx.block_tables[cache.group]
         lead = ctx.num_requests if ctx.max_q_len == 1 else ctx.leading_single

@@ -172,5 +172,5 @@ def test_items_cover_every_key_tile_of_every_token_once():
 
 def test_which_kernel_portions_take():
     take = lambda starts, lens, nq=32: kv8.reads_pages_directly(starts, lens, 0, nq, 8, 0, 148)         # noqa: E731
-    assert take([8003], [40]) and take([2000], [128]) and take([2000], [8])
-    assert not take([0], [2048]) and not take([14000], [2048]) and not take([500], [64]) and not take([], []) and not take([5], [0])
+    assert take([8003], [40]) and take([2000], [128]) and take([2000], [8]) and take([8000], [512]) and take([0], [2048])
+    assert not take([14000], [2048]) and not take([500], [64]) and not take([0], [1000]) and not take([0], [8000]) and not take([], []) and not take([5], [0])
