@@ -6,14 +6,14 @@
 //   unpack       six warps turn a tile's bytes into half precision, laid out as operands; both row tiles use what is unpacked once. By
 //                shifts and masks: the conversion instruction is as slow as the exponentials and shares their unit
 //   S = Q K^T    Q, K in shared memory (128-byte swizzle, K-major), S in tensor memory
-//   softmax      a thread has a row: it reads S from tensor memory twice (maxima; factors), 32 columns at a time, and writes factors
+//   softmax      a thread has a row: it reads S from tensor memory twice (maxima; factors), 32 columns at a time, and writes its factors
 //                over S. The loops stay short and what is rare stands outside them (masks, weights that factors do not give, values that
 //                are no number), since the instructions of four roles do not come fast enough otherwise: 2,048 tokens behind 14,000
-//                took 771 us with 64 columns a turn and all of it inside, 741 with 32, 661 so; one pass, with the rescaling inside, 846
+//                took 771 us with 64 columns a turn and all of it inside, 741 with 32, 649 so; one pass, with the rescaling inside, 744
 //   O += P V     P read from tensor memory, V in shared memory MN-major, O in tensor memory
 // While one row tile is in its softmax the tensor cores work for the other. The two tiles' S and O fill the tensor memory (512 columns).
 // What bounds it: a row tile's chain of S, maxima, factors, P V, one after another, 5,000 clocks a key tile, of them the softmax 3,100 and
-// the products 1,030. 2,048 tokens (32 heads) 66.6 us, 0.52 PFLOP/s; behind 14,000 657 us, 0.77 PFLOP/s; 40 behind 8,000 30.9 us.
+// the products 1,030. 2,048 tokens (32 heads) 66 us, 0.52 PFLOP/s; behind 14,000 649 us, 0.78 PFLOP/s; 40 behind 8,000 30.7 us.
 //
 // With t = log2(e) scale q.k and a value's scale 2^v, weights are 2^t and the factor of a value's bytes is 2^(t + v). As in
 // attention_decode_kv8_stream.cu each has its own maximum, m and mu, raised to a whole number when it is passed by more than 12: factors
@@ -489,7 +489,7 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
         const int pos_first = pos0 + tok0 + mine * P8_ROWS / G, pos_last = pos0 + tok0 + (min(rows, (mine + 1) * P8_ROWS) - 1) / G;
         float m = -INFINITY, mu = -INFINITY, l = 0.f;
         const int count = n[mine];
-        uint32_t x[32], pk[16];
+        uint32_t x[32], y[32], pk[16];
         constexpr int BLOCK = BOX;
         for (int j = 0; j < count; ++j) {
             const int j0 = (t_begin + j) * P8_KEYS;
@@ -509,10 +509,13 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
             }
             float t_top = -INFINITY, u_top = -INFINITY, v_low = INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < P8_KEYS; c += 32) {
+            for (int c = 0; c < P8_KEYS; c += 64) {
                 FA_TMEM_LD32(ts + c, x, 0);
                 p8_wait_ld(x);
+                FA_TMEM_LD32(ts + c + 32, y, 0);
                 p8_top<BLOCK>(x, of + c / 8, f, t_top, u_top, v_low);
+                p8_wait_ld(y);
+                p8_top<BLOCK>(y, of + c / 8 + 4, f, t_top, u_top, v_low);
             }
             if (t_top > m + 12.f) {
                 const float to_m = ceilf(t_top);

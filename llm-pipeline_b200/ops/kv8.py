@@ -69,7 +69,7 @@ def reads_pages_directly(starts: Sequence[int], q_lens: Sequence[int], first_req
     18 and the longer of 2.75 a key tile of the longest part and 3.2 for every key tile an SM has, against 8, 1.9 for every 1,000 tokens of
     the pages, and the longer of 2.8 a key tile of the longest item and 1.3 for every key tile an SM has, with up to 18 for the end. Measured
     (direct, unpacked), 32 query heads: 40 new tokens behind 8,000 31, 71; 128 behind 2,000 29, 48; 512 behind 8,000 113, 131; 1,024 behind
-    8,000 206, 209; 2,048 new ones 66, 70; 64 behind 500 24, 22; 1,000 new ones 35, 31; 4,000 new ones 200, 181; 2,048 behind 14,000 657, 606."""
+    8,000 206, 209; 2,048 new ones 66, 70; 64 behind 500 24, 22; 1,000 new ones 35, 31; 4,000 new ones 200, 181; 2,048 behind 14,000 649, 606."""
     group = num_heads // num_kv_heads
     wide = tiles_of(starts, q_lens, first_request, max(1, 256 // group), window)
     if not wide:
