@@ -107,6 +107,9 @@ class PromptPlan:
         self.page_size, self.window, self.dtype, self.device = page_size, window, dtype, torch.device(device)
         self.first_request = first_request
         self.rows = sum(self.q_lens)
+        # The first row where all portions are single tokens: the kernel for those takes them (behind 4,934 tokens, 3 requests of 12 and 2
+        # heads of 64: 132 us as portions, whose keys only some sizes share among blocks, 15 as single tokens).
+        self.single = sum(self.q_lens[:first_request]) if all(n == 1 for n in self.q_lens[first_request:]) else None
         self.longest = max((s + n for s, n in zip(self.starts, self.q_lens)), default=0)
         self.page_bytes = 2 * num_kv_heads * page_size * head_dim * dtype.itemsize
         self.groups = self._groups()
@@ -228,6 +231,11 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, q_stride: int, out: torc
     if not 0.0 < scale < float("inf"):                 # both ways take a row's largest score before they scale it
         raise kernels.KernelError(f"the scale of a prompt's scores must be positive and finite, not {scale}")
     if not plan.groups:
+        return out
+    if plan.single is not None:
+        at, r = plan.single, plan.first_request
+        kernels.kv8_decode_attention(q[at:plan.rows], q_stride, out[at:plan.rows], pages, block_tables[r:], ctx_len[r:], plan.longest, nq, nkv, d, ps, plan.window,
+                                     scale)
         return out
     if plan.direct() and (q.data_ptr() | 2 * q_stride | out.data_ptr()) % 16 == 0:
         items, shared, places = plan.items()

@@ -337,6 +337,20 @@ def test_portions_captured_and_replayed():
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(32, 8, 128, 16), (12, 2, 64, 16), (5, 5, 48, 8)])
+def test_portions_of_one_token_each(case, dtype):
+    """They go where single tokens go, also behind requests that are left out, and give what that gives."""
+    nq, nkv, d, ps = case
+    starts, lens, window = [10, 300, 77, 9000], [5, 1, 1, 1], 0
+    host, tables, ctx, q, out = prompt(case, starts, lens, window, dtype, 44, first=1)
+    want = torch.empty(3, nq * d, dtype=dtype, device=DEV)
+    K().kv8_decode_attention(q[5:8].to(DEV), q.stride(0), want, host.raw.to(DEV), tables[1:].to(DEV), torch.tensor(ctx[1:], dtype=torch.int32, device=DEV), 9001,
+                             nq, nkv, d, ps, window, d ** -0.5)
+    assert torch.equal(out[5:8], want) and bool((out[:5] == 9).all()) and bool((out[8:] == 9).all())
+    check_decode(host, tables[1:], q[5:8], ctx[1:], nq, nkv, d, ps, window, dtype, out[5:8], d ** -0.5)
+
+
 @pytest.mark.parametrize("direct", [True, False])
 def test_one_plan_on_two_streams(direct):
     from llm_pipeline_b200.ops import kv8
