@@ -108,7 +108,7 @@ class PromptPlan:
         self.first_request = first_request
         self.rows = sum(self.q_lens)
         # The first row where all portions are single tokens: the kernel for those takes them (behind 4,934 tokens, 3 requests of 12 and 2
-        # heads of 64: 132 us as portions, whose keys only some sizes share among blocks, 15 as single tokens).
+        # heads of 64: 132 us as portions, whose keys only some sizes share among blocks, 14 as single tokens).
         self.single = sum(self.q_lens[:first_request]) if all(n == 1 for n in self.q_lens[first_request:]) else None
         self.longest = max((s + n for s, n in zip(self.starts, self.q_lens)), default=0)
         self.page_bytes = 2 * num_kv_heads * page_size * head_dim * dtype.itemsize
