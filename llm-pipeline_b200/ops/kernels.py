@@ -14,6 +14,7 @@ import functools
 import math
 import operator
 import os
+import threading
 from typing import Optional, Sequence, Tuple
 
 import numpy as np
@@ -2401,31 +2402,40 @@ def _kv8_stream_sizes() -> Tuple[int, int]:
 
 
 _kv8_workspaces: dict = {}
+_kv8_workspaces_lock = threading.Lock()
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)     # (without the set-up check around it)
 KV8_CAPTURED_CALLS = 4096                        # captured calls with counters from the slab
 
 
+def _captured_counters(device: torch.device, count: int) -> torch.Tensor:
+    """Zeroed counters for a call that is being captured, no other call's: from the slab, or, where there is none or it is used up,
+    counters that the graph itself zeroes."""
+    with _kv8_workspaces_lock:                                   # (threads may capture at the same time)
+        slab = _kv8_workspaces.get((_device(), "slab"))
+        if slab is not None and slab[1] + count <= slab[0].numel():
+            begin, slab[1] = slab[1], slab[1] + count
+            return slab[0][begin:begin + count]
+    return torch.zeros(count, dtype=torch.int32, device=device)
+
+
 def kv8_workspace(device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
     """Scratch and zeroed counters for a launch of the streaming kernel, which leaves the counters zero. Calls on one stream follow one
-    another and share a pair. A captured call gets a pair of its own, since its graph may be replayed beside others: counters from a
-    slab that was made outside a capture, or, where there is none or it is used up, counters that the graph itself zeroes."""
-    here = _device()
+    another and share a pair. A captured call gets a pair of its own, since its graph may be replayed beside others: its counters come from a
+    slab that was made outside a capture (``_captured_counters``)."""
     if _capturing():
         floats, count = _kv8_stream_sizes()
-        scratch = torch.empty(floats, dtype=torch.float32, device=device)
-        slab = _kv8_workspaces.get((here, "slab"))
-        if slab is None or slab[1] + count > slab[0].numel():
-            return scratch, torch.zeros(count, dtype=torch.int32, device=device)
-        slab[1] += count
-        return scratch, slab[0][slab[1] - count:slab[1]]
+        return torch.empty(floats, dtype=torch.float32, device=device), _captured_counters(device, count)
+    here = _device()
     pair = _kv8_workspaces.get((here, _stream()))
     if pair is None:
         floats, count = _kv8_stream_sizes()
-        pair = _kv8_workspaces[here, _stream()] = (torch.empty(floats, dtype=torch.float32, device=device),
-                                                   torch.zeros(count, dtype=torch.int32, device=device))
-        if (here, "slab") not in _kv8_workspaces:
-            _kv8_workspaces[here, "slab"] = [torch.zeros(KV8_CAPTURED_CALLS * count, dtype=torch.int32, device=device), 0]
-            torch.cuda.current_stream().synchronize()            # nothing else orders the zeros before a replay on another stream
+        with _kv8_workspaces_lock:                               # one slab for all threads: only the books hold its memory
+            pair = _kv8_workspaces[here, _stream()] = (torch.empty(floats, dtype=torch.float32, device=device),
+                                                       torch.zeros(count, dtype=torch.int32, device=device))
+            if (here, "slab") not in _kv8_workspaces:
+                slab = torch.zeros(KV8_CAPTURED_CALLS * count, dtype=torch.int32, device=device)
+                torch.cuda.current_stream().synchronize()        # nothing else orders the zeros before a replay on another stream
+                _kv8_workspaces[here, "slab"] = [slab, 0]
     return pair
 
 
