@@ -225,12 +225,25 @@ def attention_place_floats() -> int:
 
 
 def attention_counters(device: torch.device, count: int) -> torch.Tensor:
-    """Counters with which the items that share a tile find out who finishes last; every launch leaves them zero.
-    One set per device, as for ``decode_counters``."""
+    """Counters with which the blocks that share a row's keys in the differential and the capped attention find out who
+    finishes last; every launch leaves them zero. One set per device, as for ``decode_counters``."""
     key = torch.device(device).index or 0
     counters = _attention_counters.get(key)
     if counters is None or counters.numel() < count:
         _need(not torch.cuda.is_current_stream_capturing(), "attention counters must exist before a graph is captured")
+        counters = _attention_counters[key] = torch.zeros(max(count, 65536), dtype=torch.int32, device=device)
+    return counters
+
+
+def shared_tile_counters(device: torch.device, count: int) -> torch.Tensor:
+    """Counters with which the items that share a tile's keys in ``paged_attention`` find out who finishes last; every launch
+    leaves them zero. One set per stream, whose launches follow one another; a captured call has counters of its own, since its
+    graph may be replayed beside other calls."""
+    if _capturing():
+        return _captured_counters(device, count)
+    key = (_device(), _stream())
+    counters = _attention_counters.get(key)
+    if counters is None or counters.numel() < count:
         counters = _attention_counters[key] = torch.zeros(max(count, 65536), dtype=torch.int32, device=device)
     return counters
 
@@ -676,7 +689,7 @@ def paged_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, pages: to
         _need(tile_seg.numel() == tile_req.numel() == tile_slot.numel() and 0 < places <= ATTENTION_MAX_PLACES,
               "tile_seg and tile_slot must have an entry per item, and the places a count within bounds")
         partials = torch.empty(places * num_kv_heads * attention_place_floats(), dtype=torch.float32, device=q.device)
-        counters = attention_counters(q.device, places * num_kv_heads)
+        counters = shared_tile_counters(q.device, places * num_kv_heads)
         seg, slot = tile_seg, tile_slot
     _call("llmp_paged_attention", _ptr(q), int(q_stride), _ptr(out), out.stride(0), _ptr(pages), pages.shape[0],
           dtype_code(q.dtype), _ptr(block_tables), block_tables.stride(0), _ptr(q_start), _ptr(ctx_len),
