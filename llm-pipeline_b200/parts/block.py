@@ -7,6 +7,8 @@ on the stream and the next norm kernel adds it into the float32 residual."""
 
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 
 from ..cache.spec import StateSpec
@@ -147,7 +149,7 @@ class ParallelResidualBlock(Block):
         h_mixer, h_ff = self._inputs(stream, ctx, cache)
         if self._own_state:
             state = cache.state[:, self._own_state:] if self._mixer_state is not None else None
-            cache = LayerCache(pages=cache.pages, group=cache.group, state=state, writes=cache.writes)
+            cache = replace(cache, state=state)
         out, bias = self.mixer.forward(h_mixer, ctx, cache)
         stream.add(out, bias)
         if self.feed_forward is not None:

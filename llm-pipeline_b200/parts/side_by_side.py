@@ -10,6 +10,7 @@ two products are one. A block that takes addends gets both results with their no
 
 from __future__ import annotations
 
+from dataclasses import replace
 from typing import Any, Dict, List, Optional, Sequence
 
 import torch
@@ -110,8 +111,7 @@ class SideBySide(Mixer):
         at = 0
         for m, span in zip(self.members, self._state_at):
             state = cache.state[:, span[0]:span[1]] if span is not None and cache.state is not None else None
-            view = LayerCache(pages=cache.pages if m.cache_spec() is not None else None, group=cache.group, state=state,
-                              writes=cache.writes)
+            view = replace(cache, pages=cache.pages if m.cache_spec() is not None else None, state=state)
             if proj is not None:
                 out, bias = m.forward_from(proj[:, at:at + m.w_in.shape[0]], ctx, view)
                 at += m.w_in.shape[0]
