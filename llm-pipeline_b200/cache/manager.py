@@ -302,7 +302,9 @@ class CacheManager:
         """Requests ``new_ids`` that begin with the first ``length`` tokens of a live one (None: all it has): they hold its full
         pages with it, copies of the page that is filled in part, and copies of its state. All or nothing; False when slots
         or pages are too few. A request with state can only be forked at its present length, one whose window has moved on not before
-        what the window still holds. The copies are queued behind the steps that are issued, on the current stream."""
+        what the window still holds. The copies are queued behind the steps that are issued, on the current stream. Pages in 8 bits are copied as
+        they are: inside a page, before its last token, the new requests hold what the parent's later tokens made of its scales and
+        roundings (``fork_length`` gives a length without such tokens)."""
         if req_id not in self._requests:
             raise CacheError(f"request {req_id!r} is not live")
         parent, new_ids = self._requests[req_id], list(new_ids)
@@ -345,6 +347,12 @@ class CacheManager:
             if new_ids:
                 copy_pages(tensors, [parent.slot] * len(slots), slots)
         return True
+
+    def fork_length(self, req_id: Hashable, length: int) -> int:
+        """The largest length, at most ``length``, at which a fork holds nothing of what the request holds behind it: a page's
+        scale in 8 bits, and the roundings it brings, follow from all tokens of the page."""
+        inside = length < self.length(req_id) and any(group.spec.scaled_by_page for group in self.groups)
+        return length - length % self.page_size if inside else length
 
     def compact(self) -> int:
         """Move the pages in use to the lowest page ids, so that the free ones are one run at the end; returns how many

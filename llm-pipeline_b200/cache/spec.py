@@ -35,6 +35,7 @@ class PagesSpec:
     keep_first: int = 0                          # tokens at a request's start that a window never leaves behind
     chunk: Optional[int] = None                  # tokens see the keys of their own chunk of this many tokens
     dtype: Optional[torch.dtype] = None          # None: the element type the cache was made with
+    scaled_by_page = False                       # what a page holds of a token follows from the page's later tokens too
 
     def page_shape(self, page_size: int) -> Tuple[int, ...]:
         raise NotImplementedError
@@ -98,6 +99,7 @@ class KV8PagesSpec(PagesSpec):
     head_dim: int
     window: Optional[int] = None
     dtype = torch.uint8
+    scaled_by_page = True
 
     def page_shape(self, page_size: int) -> Tuple[int, ...]:
         return (kv8_page_bytes(self.num_kv_heads, page_size, self.head_dim),)

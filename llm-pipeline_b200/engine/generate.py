@@ -128,6 +128,8 @@ class GenerationEngine:
                 continue
             waiting = self._forks.pop(first.req_id)
             shared = len(first.prompt) - 1
+            if entry.start + entry.count > len(first.prompt):        # read again after a preemption, what it had sampled along with it
+                shared = self.cache.fork_length(first.req_id, shared)
             room = min(len(waiting), self.scheduler.max_num_seqs - len(self.scheduler.running), self.cache.free_slots)
             now = waiting[:max(room, 0)] if shared else []
             if now and self.cache.fork(first.req_id, [r.req_id for r in now], shared):

@@ -55,3 +55,41 @@ def test_portions_whose_keys_are_shared_run_beside_one_another(direct, how):
     torch.cuda.synchronize()
     for (want, _call, _plan), got in zip(sets, outs):
         assert all(torch.equal(out, want) for out in got)
+
+
+@pytest.mark.parametrize("length", [13, 16, 29, 40])
+def test_a_fork_at_the_length_that_is_offered_holds_its_own_tokens_alone(length):
+    """The parent's later tokens are a thousand times larger: the fork, once it has stored its tokens, holds what a request that never shared
+    anything holds."""
+    from llm_pipeline_b200.cache import CacheManager, KV8PagesSpec
+    from llm_pipeline_b200.ops import kernels
+
+    nkv, d, ps, N = 2, 32, 16, 40
+    cache = CacheManager([(KV8PagesSpec(nkv, d), None)], page_size=ps, num_pages=16, max_requests=4, max_request_tokens=64, device=torch.device(DEV))
+    pages = cache.pages_tensor(0)
+    x = torch.randn(64, 2 * nkv * d, generator=torch.Generator().manual_seed(3)).bfloat16().to(DEV)
+
+    def store(rid, begin, end, factor=1.0):
+        assert cache.reserve(rid, end)
+        table = cache.block_table(rid, 0)
+        slots = torch.tensor([table[t // ps] * ps + t % ps for t in range(begin, end)], dtype=torch.int32, device=DEV)
+        rows = x[begin:end] * factor
+        kernels.kv8_store(rows[:, :nkv * d], rows[:, nkv * d:], slots, pages, nkv, d, ps)
+        cache.commit(rid, end)
+
+    cache.admit("parent")
+    store("parent", 0, length)
+    if length < N:
+        store("parent", length, N, 1000.0)
+    at = cache.fork_length("parent", length)
+    assert at == (length if length == N else length - length % ps) and cache.fork("parent", ["child"], at)
+    cache.admit("alone")
+    for rid, begin in (("child", at), ("alone", 0)):
+        store(rid, begin, length)
+        store(rid, length, length + 2)
+    body = 2 * nkv * ps * d
+    for n, (a, b) in enumerate(zip(cache.block_table("child", 0), cache.block_table("alone", 0))):
+        one, other = pages[a], pages[b]
+        assert torch.equal(one[body:body + 2 * nkv], other[body:body + 2 * nkv])
+        there = min(ps, length + 2 - n * ps)
+        assert torch.equal(one[:body].view(2 * nkv, ps, d)[:, :there], other[:body].view(2 * nkv, ps, d)[:, :there])
