@@ -132,10 +132,11 @@ class GenerationEngine:
                 shared = self.cache.fork_length(first.req_id, shared)
             room = min(len(waiting), self.scheduler.max_num_seqs - len(self.scheduler.running), self.cache.free_slots)
             now = waiting[:max(room, 0)] if shared else []
-            if now and self.cache.fork(first.req_id, [r.req_id for r in now], shared):
-                for request in now:
-                    self.scheduler.add_forked(request, shared)
-                waiting = waiting[len(now):]
+            while now and not self.cache.fork(first.req_id, [r.req_id for r in now], shared):
+                now.pop()                                        # (as many as there are pages for)
+            for request in now:
+                self.scheduler.add_forked(request, shared)
+            waiting = waiting[len(now):]
             for request in waiting:
                 self.scheduler.add(request)
 

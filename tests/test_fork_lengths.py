@@ -78,3 +78,31 @@ def test_a_short_prompt_of_a_preempted_request_is_computed_again():
     e.add_request(range(3), 9, req_id="b", same_prompt_as="a")
     assert step(e) == {"a": (0, 5)}
     assert step(e) == {"a": (5, 1), "b": (0, 3)}
+
+
+@pytest.mark.parametrize("specs", [BF16, EIGHT])
+def test_as_many_share_a_prompt_as_there_are_pages_for(specs):
+    """22 tokens are six pages, two tokens of the last. Six free pages are not enough for seven copies of that page: six requests share."""
+    e = engine(specs, num_pages=12)
+    e.add_request(range(22), 3, req_id="a")
+    for i in range(7):
+        e.add_request(range(22), 3, req_id=i, same_prompt_as="a")
+    assert step(e) == {"a": (0, 22)}
+    shared = [i for i in range(7) if i in e.cache]
+    assert shared == [0, 1, 2, 3, 4, 5] and e.cache.groups[0].pool.num_free == 0
+    computed = 22 + sum(n for _s, n in step(e).values())
+    while e.scheduler.has_unfinished():
+        computed += sum(n for _s, n in step(e).values())
+    assert all(r.output == [7] * 3 for r in e._requests.values()) and e.cache.num_live == 0 and not e._forks
+    assert computed < 4 * 22
+
+
+def test_none_share_where_no_page_is_left():
+    e = engine(EIGHT, num_pages=6)
+    e.add_request(range(22), 2, req_id="a")
+    e.add_request(range(22), 2, req_id="b", same_prompt_as="a")
+    assert step(e) == {"a": (0, 22)}
+    assert "b" not in e.cache
+    while e.scheduler.has_unfinished():
+        step(e)
+    assert e._requests["b"].output == [7, 7] and e.cache.num_live == 0
