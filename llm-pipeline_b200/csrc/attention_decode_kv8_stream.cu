@@ -622,7 +622,7 @@ decode_kv8_stream_kernel(const __grid_constant__ CUtensorMap map, const Stream8P
 // Sizes the kernel takes (bfloat16 queries whose rows start on 16 bytes), the scratch it needs and its counters, which are zero before
 // a launch and after it; launches that may run at the same time need scratch and counters of their own.
 LLMP_API int llmp_kv8_stream_supports(int nq, int nkv, int d, int page_size) {
-    return d == S8_D && nkv > 0 && nq % nkv == 0 && page_size >= 8 && (page_size & (page_size - 1)) == 0;
+    return d == S8_D && nq > 0 && nkv > 0 && nq % nkv == 0 && page_size >= 8 && (page_size & (page_size - 1)) == 0;
 }
 LLMP_API long llmp_kv8_stream_scratch_floats() { return (long)S8_MAX_BLOCKS * 2 * S8_PART; }
 LLMP_API int llmp_kv8_stream_counters() { return S8_MAX_BLOCKS; }

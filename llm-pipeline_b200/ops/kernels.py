@@ -129,7 +129,7 @@ _SIGNATURES = {
     "llmp_kv8_gather": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P],
     "llmp_kv8_decode": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
     "llmp_kv8_stream": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P, _P],
-    "llmp_kv8_prompt": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P],
+    "llmp_kv8_prompt": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P],
     "llmp_copy_pages": [_P, _I, _L, _P, _P, _I, _P],
 }
 _bound = {}
@@ -2508,18 +2508,33 @@ def kv8_prompt_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
                          page_size: int, window: int, scale: float) -> torch.Tensor:
     """Causal attention of a step's query rows (head size 128) over 8-bit pages. ``items`` int32 [n, 4]: request, first token, number of a
     part of the tile's keys | parts << 16, place of the part's sums; ``shared`` int32 [m, 4]: request, first token, parts, first place of
-    every tile that comes in parts (``ops.kv8.PromptPlan`` makes both)."""
+    every tile that comes in parts (``ops.kv8.PromptPlan`` makes both; what they hold is not checked). Rows that q or out does not have are
+    left out."""
+    if not kv8_prompt_supports(q.dtype, num_heads, num_kv_heads, 128, page_size):
+        if q.dtype != torch.bfloat16:
+            raise KernelError("prompt attention over 8-bit pages takes bfloat16 queries")
+        raise KernelError(f"the kernel over 8-bit pages does not serve {num_heads} and {num_kv_heads} heads and pages of {page_size} tokens")
     for name, t in (("block_tables", block_tables), ("q_start", q_start), ("ctx_len", ctx_len), ("items", items), ("shared", shared)):
         _i32(t, name)
     if not (items.dim() == shared.dim() == 2 and items.shape[1] == shared.shape[1] == 4):
         raise KernelError("the lists of a prompt's items must be [n, 4]")
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.shape[1] != num_heads * 128:
-        raise KernelError("prompt attention over 8-bit pages takes bfloat16 queries and gives contiguous bfloat16 [tokens, heads * 128]")
+    if places < 0 or (places > 0) != (shared.shape[0] > 0):
+        raise KernelError(f"{shared.shape[0]} shared tiles do not go with {places} places for their sums")
+    shape, width = q.shape, num_heads * 128
+    if len(shape) != 2 or shape[1] < width or q.stride(1) != 1 or (shape[0] > 1 and q.stride(0) != q_stride):
+        raise KernelError("query rows must be [tokens, at least heads * 128] and lie q_stride apart")
+    if out.dtype != torch.bfloat16 or not out.is_contiguous() or out.dim() != 2 or out.shape[1] != width:
+        raise KernelError("prompt attention over 8-bit pages gives contiguous bfloat16 [tokens, heads * 128]")
+    R, table = ctx_len.numel(), block_tables.shape
+    if len(table) != 2 or table[0] != R or table[1] == 0 or q_start.numel() != R + 1:
+        raise KernelError("block tables must be [requests, pages], ctx_len and q_start those of the same requests")
+    if window < 0 or not math.isfinite(scale):
+        raise KernelError("the window must not be negative, the scale finite")
     _kv8_pages(pages, num_kv_heads, 128, page_size)
     _on_current_device(q, out, pages, block_tables, q_start, ctx_len, items, shared)
     partials = torch.empty(places * kv8_prompt_sizes(num_heads, num_kv_heads)[1], dtype=torch.float32, device=q.device) if places else None
-    _call("llmp_kv8_prompt", q.data_ptr(), q_stride, out.data_ptr(), out.stride(0), pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
-          block_tables.shape[1], q_start.data_ptr(), ctx_len.data_ptr(), items.data_ptr(), items.shape[0], shared.data_ptr() if places else None,
+    _call("llmp_kv8_prompt", q.data_ptr(), q_stride, out.data_ptr(), width, min(shape[0], out.shape[0]), pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
+          table[1], q_start.data_ptr(), ctx_len.data_ptr(), items.data_ptr(), items.shape[0], shared.data_ptr() if places else None,
           shared.shape[0], None if partials is None else partials.data_ptr(), num_heads, num_kv_heads, page_size, window, scale,
           error_flag().data_ptr(), _stream())
     return out

@@ -100,6 +100,8 @@ class PromptPlan:
                  window: int, dtype: torch.dtype, device: torch.device, first_request: int = 0):
         if len(starts) != len(q_lens) or any(n < 0 for n in q_lens) or any(s < 0 for s in starts):
             raise kernels.KernelError("a plan needs the cached and the new tokens of every request")
+        if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
+            raise kernels.KernelError(f"{num_heads} query heads cannot share {num_kv_heads} key/value heads")
         if page_size <= 0 or window < 0 or not 0 <= first_request <= len(q_lens):
             raise kernels.KernelError("a plan needs a positive page size, a window of at least 0 and a first request of the step")
         self.starts, self.q_lens = [int(s) for s in starts], [int(n) for n in q_lens]
