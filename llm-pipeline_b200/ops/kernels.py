@@ -2509,7 +2509,7 @@ def kv8_prompt_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
     """Causal attention of a step's query rows (head size 128) over 8-bit pages. ``items`` int32 [n, 4]: request, first token, number of a
     part of the tile's keys | parts << 16, place of the part's sums; ``shared`` int32 [m, 4]: request, first token, parts, first place of
     every tile that comes in parts (``ops.kv8.PromptPlan`` makes both; what they hold is not checked). Rows that q or out does not have are
-    left out."""
+    left out. The scale may have any sign (``ops.kv8.prompt_attention``, which may go over unpacked pages, takes positive ones only)."""
     if not kv8_prompt_supports(q.dtype, num_heads, num_kv_heads, 128, page_size):
         if q.dtype != torch.bfloat16:
             raise KernelError("prompt attention over 8-bit pages takes bfloat16 queries")

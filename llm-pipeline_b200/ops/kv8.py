@@ -230,7 +230,7 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, q_stride: int, out: torc
         raise kernels.KernelError("the plan has more rows than the queries or the output")
     if block_tables.shape[1] * ps < plan.longest:
         raise kernels.KernelError(f"a request sees {plan.longest} tokens, its block table has room for {block_tables.shape[1] * ps}")
-    if not 0.0 < scale < float("inf"):                 # both ways take a row's largest score before they scale it
+    if not 0.0 < scale < float("inf"):                 # (the kernel over ordinary pages takes a row's largest score before it scales it)
         raise kernels.KernelError(f"the scale of a prompt's scores must be positive and finite, not {scale}")
     if not plan.groups:
         return out

@@ -93,3 +93,35 @@ def test_a_fork_at_the_length_that_is_offered_holds_its_own_tokens_alone(length)
         assert torch.equal(one[body:body + 2 * nkv], other[body:body + 2 * nkv])
         there = min(ps, length + 2 - n * ps)
         assert torch.equal(one[:body].view(2 * nkv, ps, d)[:, :there], other[:body].view(2 * nkv, ps, d)[:, :there])
+
+
+@pytest.mark.parametrize("scale", [-0.09, 0.0, 0.09])
+@pytest.mark.parametrize("starts,lens", [([300, 0], [40, 150]), ([4000], [9])])
+def test_the_kernel_that_reads_pages_takes_scales_of_any_sign(scale, starts, lens):
+    """Called by itself; over unpacked pages a scale has to be positive, so that a step's portions refuse others."""
+    import kv8_plain as plain
+    from llm_pipeline_b200.ops import kernels, kv8
+    from test_gpu_kv8 import bound
+
+    nq, nkv, d, ps = 32, 8, 128, 16
+    host, tables, ctx, q, _out = prompt((nq, nkv, d, ps), starts, lens, 0, torch.bfloat16, 55)
+    plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, 0, torch.bfloat16, torch.device(DEV))
+    items, shared, places = plan.items()
+    N = sum(lens)
+    out = torch.full((N + 2, nq * d), 9.0, dtype=torch.bfloat16, device=DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)               # noqa: E731
+    start, ct = i32([sum(lens[:r]) for r in range(len(lens) + 1)]), i32(ctx)
+    kernels.kv8_prompt_attention(q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV), start, ct, items, shared, places, nq, nkv, ps, 0, scale)
+    at = 0
+    for r, n in enumerate(lens):
+        k, v, there = host.request(tables[r], ctx[r])
+        for i in sorted({0, n // 2, n - 1}):
+            seen = slice(0, starts[r] + i + 1)
+            row = q[at + i:at + i + 1, :nq * d].view(1, nq, d)
+            want, size, top = plain.attend(row, k[seen], v[seen], [starts[r] + i], there[seen], scale, 0)
+            # (`smallest` as for single tokens: weights times the values' scales in half precision)
+            allowed = bound(want, size, top.abs(), torch.bfloat16, d) + plain.smallest(row[0], k[seen], v[seen], host.value_scales(tables[r], ctx[r])[seen],
+                                                                                      starts[r] + i, there[seen], scale, 0)
+            assert bool(((out[at + i].double().cpu().view(1, nq, d) - want).abs() <= allowed).all()), (r, i)
+        at += n
+    assert bool((out[N:] == 9).all())
