@@ -143,11 +143,9 @@ __global__ void __launch_bounds__(ATT_THREADS) paged_attention_kernel(const Attn
             const float s = Ss[rr * (ATT_KEYS + 1) + lane];
             const float m_old = row_m[rr];
             const float m_new = fmaxf(m_old, warp_max(s));
-            float pr = 0.f, alpha = 1.f;
-            if (m_new > -INFINITY) {
-                pr = expf(s - m_new);          // exp(-inf) = 0 for masked keys
-                alpha = expf(m_old - m_new);   // 0 when nothing was seen before
-            }
+            // masked keys have weight 0; a score that is no number keeps its own, also where none of the row is a number
+            const float pr = s == -INFINITY ? 0.f : expf(s - (m_new > -INFINITY ? m_new : 0.f));
+            const float alpha = m_new > -INFINITY ? expf(m_old - m_new) : 1.f;      // 0 when nothing was seen before
             const float sum = warp_sum(pr);
             Ss[rr * (ATT_KEYS + 1) + lane] = pr;
             __syncwarp();
@@ -177,7 +175,7 @@ __global__ void __launch_bounds__(ATT_THREADS) paged_attention_kernel(const Attn
         const int tl = tok0 + rr / p.heads_per_cta, hh = head0 + rr % p.heads_per_cta;
         if (rr < rows && tl < q_len && hh < G) {
             const float l = row_l[rr];
-            const float v = l > 0.f ? Os[e] / l : 0.f;
+            const float v = l != 0.f ? Os[e] / l : 0.f;           // no keys: zeros
             out[(size_t)(q_begin + tl) * p.out_stride + (size_t)(kvh * G + hh) * d + c] = from_float<T>(v);
         }
     }

@@ -125,3 +125,34 @@ def test_the_kernel_that_reads_pages_takes_scales_of_any_sign(scale, starts, len
             assert bool(((out[at + i].double().cpu().view(1, nq, d) - want).abs() <= allowed).all()), (r, i)
         at += n
     assert bool((out[N:] == 9).all())
+
+
+@pytest.mark.parametrize("direct", [True, False])
+@pytest.mark.parametrize("nq,nkv,d,ps,starts,lens", [(32, 8, 128, 16, [0, 100], [70, 5]), (6, 2, 80, 8, [100], [60]), (6, 3, 256, 16, [100], [40])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_queries_and_keys_that_are_no_numbers_do_not_come_out_as_zeros(nq, nkv, d, ps, starts, lens, dtype, direct):
+    """A query with a NaN: its own row. A key with one: the rows that see it. Whatever else the row sees, nothing at all included."""
+    from llm_pipeline_b200.ops import kernels, kv8
+
+    if direct and not kernels.kv8_prompt_supports(dtype, nq, nkv, d, ps):
+        pytest.skip("no kernel reads these pages as they are")
+    G, N = nq // nkv, sum(lens)
+    host, tables, ctx, q, clean = prompt((nq, nkv, d, ps), starts, lens, 0, dtype, 84, direct=direct)
+    q[3, (nq - 1) * d + 5] = float("nan")
+    q[N - 1, 2] = float("nan")
+    token = starts[0] + 20 if starts[0] else 0                                   # the first token of all: its row sees nothing else
+    host.q[int(tables[0, token // ps]), 0, 1, token % ps, d - 1] = 127
+    want = torch.zeros(N + 2, nq, dtype=torch.bool)
+    want[3, nq - 1] = want[N - 1, 0] = True
+    for i in range(lens[0]):
+        if starts[0] + i >= token:
+            want[i, G:2 * G] = True
+    out = torch.full_like(clean, 9.0)
+    plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, 0, dtype, torch.device(DEV))
+    plan._direct = direct
+    kv8.prompt_attention(plan, q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV),
+                         torch.tensor([sum(lens[:r]) for r in range(len(lens) + 1)], dtype=torch.int32, device=DEV),
+                         torch.tensor(ctx, dtype=torch.int32, device=DEV), d ** -0.5)
+    got = out.view(-1, nq, d).cpu()
+    assert torch.equal(got.isnan().all(-1), want)
+    assert torch.equal(got[~want], clean.view(-1, nq, d).cpu()[~want])
