@@ -397,8 +397,10 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_pages, const
                 }
 #pragma unroll
                 for (int x = 0; x < FA_MAX_SEGMENTS; ++x) {
-                    wgt[x] = wgt[x] > -INFINITY ? fa_ex2(wgt[x] - m) : 0.f;
-                    if (x < nseg && wgt[x] != 0.f) l = fmaf(__ldcg(first + (size_t)x * p.nkv * FA_PART + FA_ROWS * FA_D + FA_ROWS + tid), wgt[x], l);
+                    // (an item without a maximum saw no key, its sum is 0, or none whose score is a number: that sum counts)
+                    const float sum = x < nseg ? __ldcg(first + (size_t)x * p.nkv * FA_PART + FA_ROWS * FA_D + FA_ROWS + tid) : 0.f;
+                    wgt[x] = wgt[x] > -INFINITY ? fa_ex2(wgt[x] - m) : (sum != 0.f ? 1.f : 0.f);
+                    if (wgt[x] != 0.f) l = fmaf(sum, wgt[x], l);
                 }
                 const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1

@@ -128,7 +128,8 @@ def test_the_kernel_that_reads_pages_takes_scales_of_any_sign(scale, starts, len
 
 
 @pytest.mark.parametrize("direct", [True, False])
-@pytest.mark.parametrize("nq,nkv,d,ps,starts,lens", [(32, 8, 128, 16, [0, 100], [70, 5]), (6, 2, 80, 8, [100], [60]), (6, 3, 256, 16, [100], [40])])
+@pytest.mark.parametrize("nq,nkv,d,ps,starts,lens", [(32, 8, 128, 16, [5000], [40]), (32, 8, 128, 16, [0, 100], [70, 5]), (6, 2, 80, 8, [100], [60]),
+                                                     (6, 3, 256, 16, [100], [40])])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_queries_and_keys_that_are_no_numbers_do_not_come_out_as_zeros(nq, nkv, d, ps, starts, lens, dtype, direct):
     """A query with a NaN: its own row. A key with one: the rows that see it. Whatever else the row sees, nothing at all included."""
