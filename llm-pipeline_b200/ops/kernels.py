@@ -126,7 +126,7 @@ _SIGNATURES = {
     "llmp_xielu": [_P, _P, _I, _F, _F, _P, _I, _L, _I, _P],
     "llmp_scaled_sum": [_P, _F, _P, _F, _P, _L, _P],
     "llmp_kv8_store": [_P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _I, _P],
-    "llmp_kv8_gather": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P],
+    "llmp_kv8_gather": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P],
     "llmp_kv8_decode": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
     "llmp_kv8_stream": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P, _P],
     "llmp_kv8_prompt": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P],
@@ -2369,10 +2369,12 @@ def kv8_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pages: torc
           num_kv_heads, head_dim, page_size, _stream())
 
 
-def kv8_gather(pages: torch.Tensor, block_tables: torch.Tensor, ctx_len: torch.Tensor, index: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+def kv8_gather(pages: torch.Tensor, block_tables: torch.Tensor, ctx_len: torch.Tensor, index: torch.Tensor, out: torch.Tensor,
+               hide: bool = False) -> torch.Tensor:
     """out[i] (``[n, 2, kv heads, page_size, head_dim]``, float32 or bfloat16, exact in either) = the values of the 8-bit page
     that entry ``index[i]`` of the flattened ``block_tables`` names; zeros behind the request's last token and for a page that
-    is missing."""
+    is missing. ``hide``, for attention kernels that multiply what a row does not see by 0: a value that is no number becomes 0, and all
+    keys of its token and head become no numbers in its place, which masks keep from the rows that do not see the token."""
     shape, table = out.shape, block_tables.shape
     if len(shape) != 5 or shape[1] != 2 or not out.is_contiguous():
         raise KernelError("unpacked pages must be contiguous [n, 2, kv heads, page_size, head_dim]")
@@ -2388,7 +2390,7 @@ def kv8_gather(pages: torch.Tensor, block_tables: torch.Tensor, ctx_len: torch.T
     dtype = dtype_code(out.dtype)
     _on_current_device(pages, block_tables, ctx_len, index, out)
     _call("llmp_kv8_gather", pages.data_ptr(), P, block_tables.data_ptr(), table[0], table[1], ctx_len.data_ptr(),
-          index.data_ptr(), n, out.data_ptr(), dtype, nkv, d, page_size, _stream())
+          index.data_ptr(), n, out.data_ptr(), dtype, nkv, d, page_size, int(hide), _stream())
     return out
 
 

@@ -4,8 +4,8 @@ bfloat16 queries of head size 128 go to a kernel that reads the pages as they ar
 faster: few queries over many keys above all (``reads_pages_directly``). For all others the pages that a step's portions see are
 unpacked into a workspace of the query's type, laid out as ordinary pages, and the attention kernels of ordinary pages run over it
 (``kernels.paged_attention``): a page's values are exact in either type (the scales are powers of two), so the result is exactly what
-they give for a cache that holds these values. A value that is no number makes the whole rows of a head that see it no numbers in the
-one kernel, their entry of the value's column in the others."""
+they give for a cache that holds these values. A value that is no number makes the whole rows of its head's group that see its token no
+numbers either way, and no others (single tokens: the entries of its column)."""
 
 from __future__ import annotations
 
@@ -248,7 +248,7 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, q_stride: int, out: torc
     for index, tables, req, tok0, seg, slot, places, tokens in plan.lists(block_tables.shape[1]):
         plan._for_this_stream((index, tables, req, tok0, seg, slot))
         held = torch.empty((index.numel(), 2, nkv, ps, d), dtype=q.dtype, device=q.device)
-        kernels.kv8_gather(pages, block_tables, ctx_len, index, held)
+        kernels.kv8_gather(pages, block_tables, ctx_len, index, held, hide=True)
         kernels.paged_attention(q, q_stride, out, held, tables, q_start, ctx_len, req, tok0, nq, nkv, d, ps, plan.window, scale, tokens,
                                 seg, slot, places)
     return out

@@ -128,6 +128,43 @@ def test_the_kernel_that_reads_pages_takes_scales_of_any_sign(scale, starts, len
 
 
 @pytest.mark.parametrize("direct", [True, False])
+@pytest.mark.parametrize("nq,nkv,d,ps,starts,lens,window", [(8, 2, 128, 16, [200], [300], 150), (32, 8, 128, 16, [5000, 0], [40, 200], 0), (9, 1, 128, 64, [700], [70], 0),
+                                                            (16, 8, 128, 8, [3000], [3], 2500), (8, 8, 128, 128, [0], [257], 0), (6, 2, 80, 8, [100], [200], 0),
+                                                            (6, 3, 256, 16, [100], [40], 0), (4, 4, 16, 4, [90], [90], 60)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_value_that_is_no_number_reaches_the_rows_that_see_its_token(nq, nkv, d, ps, starts, lens, window, dtype, direct):
+    """A NaN among a head's values makes the rows of its group that see the token no numbers, and leaves all others, those of earlier
+    tokens and of later windows in the same call among them, as they are to the bit: in every kernel that portions may go to."""
+    from llm_pipeline_b200.ops import kernels, kv8
+
+    if direct and not kernels.kv8_prompt_supports(dtype, nq, nkv, d, ps):
+        pytest.skip("no kernel reads these pages as they are")
+    G = nq // nkv
+    host, tables, ctx, q, clean = prompt((nq, nkv, d, ps), starts, lens, window, dtype, 83, direct=direct)
+    end = ctx[0] - 1
+    # (token, key/value head, column, byte): both signs, first and last columns, tokens of one page and far apart
+    values = [(end - 2, 0, 7, 127), (end - 2, 0, d - 1, 255), (end - 33, nkv - 1, 0, 127), (max(end - 140, starts[0] + 1), nkv - 1, d // 2, 255)]
+    for t, h, c, byte in values:
+        host.q[int(tables[0, t // ps]), 1, h, t % ps, c] = byte
+    want = torch.zeros(sum(lens) + 2, nq, dtype=torch.bool)
+    for i in range(lens[0]):
+        pos = starts[0] + i
+        for t, h, _c, _byte in values:
+            if t <= pos and (not window or t > pos - window):
+                want[i, h * G:(h + 1) * G] = True
+    out = torch.full_like(clean, 9.0)
+    plan = kv8.PromptPlan(starts, lens, nq, nkv, d, ps, window, dtype, torch.device(DEV))
+    plan._direct = direct
+    kv8.prompt_attention(plan, q.to(DEV), q.stride(0), out, host.raw.to(DEV), tables.to(DEV),
+                         torch.tensor([sum(lens[:r]) for r in range(len(lens) + 1)], dtype=torch.int32, device=DEV),
+                         torch.tensor(ctx, dtype=torch.int32, device=DEV), d ** -0.5)
+    got = out.view(-1, nq, d).cpu()
+    assert bool(want.any()) and not bool(want[:lens[0]].all())
+    assert torch.equal(got.isnan().all(-1), want)
+    assert torch.equal(got[~want], clean.view(-1, nq, d).cpu()[~want])
+
+
+@pytest.mark.parametrize("direct", [True, False])
 @pytest.mark.parametrize("nq,nkv,d,ps,starts,lens", [(32, 8, 128, 16, [5000], [40]), (32, 8, 128, 16, [0, 100], [70, 5]), (6, 2, 80, 8, [100], [60]),
                                                      (6, 3, 256, 16, [100], [40])])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
