@@ -194,3 +194,40 @@ def test_queries_and_keys_that_are_no_numbers_do_not_come_out_as_zeros(nq, nkv, 
     got = out.view(-1, nq, d).cpu()
     assert torch.equal(got.isnan().all(-1), want)
     assert torch.equal(got[~want], clean.view(-1, nq, d).cpu()[~want])
+
+
+@pytest.mark.parametrize("nkv,d,ps", [(2, 128, 16), (3, 48, 24), (1, 256, 8), (8, 16, 4), (2, 80, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_storing_many_rows_of_ragged_portions(nkv, d, ps, dtype):
+    """A thousand rows and more: portions that begin and end anywhere in a page and in a block's rows, single tokens between them, rows without a
+    slot, first, last, inside runs and many of them together."""
+    import kv8_plain as plain
+    from llm_pipeline_b200.ops import kernels
+    from test_gpu_kv8 import filled, same_bytes
+
+    gen = torch.Generator().manual_seed(ps + d)
+    pick = lambda low, high: int(torch.randint(low, high + 1, (1,), generator=gen))      # noqa: E731
+    slots, page = [-1, -1], 0
+    while len(slots) < 1300:
+        kind, offset = pick(0, 5), pick(0, ps - 1)
+        if kind == 0:
+            slots += [-1] * pick(1, 40)
+        elif kind == 1:
+            slots.append(page * ps + offset)
+            page += 1
+        else:
+            n = pick(1, 5 * ps)
+            run = [page * ps + offset + i for i in range(n)]
+            if kind == 2:
+                run.insert(n // 2, -1)
+            slots += run
+            page = run[-1] // ps + 1
+    slots += [-1] * 35
+    host = filled(page + 1, nkv, ps, d, 6)
+    pages = host.raw.to(DEV)
+    x = (torch.randn(len(slots), 2 * nkv * d, generator=gen) * torch.exp(2.0 * torch.randn(len(slots), 1, generator=gen))).to(dtype)
+    host.store(x[:, :nkv * d], x[:, nkv * d:], slots)
+    on = x.to(DEV)
+    kernels.kv8_store(on[:, :nkv * d], on[:, nkv * d:], torch.tensor(slots, dtype=torch.int32, device=DEV), pages, nkv, d, ps)
+    same_bytes(pages, host.raw)
+    assert plain.page_bytes(nkv, ps, d) == pages.shape[1]
