@@ -288,6 +288,7 @@ class GenerationEngine:
     def stats(self) -> Dict[str, object]:
         out = {"steps": self.steps, "tokens_prefilled": self.tokens_prefilled, "tokens_decoded": self.tokens_decoded}
         out.update(self.scheduler.stats())
+        out["waiting"] += sum(map(len, self._forks.values()))        # those that wait for another request's prompt
         out.update(self.cache.stats())
         if self.runner.kernel_times is not None:             # LLMP_B200_KERNEL_TIMES=1
             out["kernel_times"] = self.runner.kernel_times.table()

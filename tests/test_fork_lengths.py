@@ -106,3 +106,17 @@ def test_none_share_where_no_page_is_left():
     while e.scheduler.has_unfinished():
         step(e)
     assert e._requests["b"].output == [7, 7] and e.cache.num_live == 0
+
+
+def test_requests_that_wait_for_a_prompt_are_counted_as_waiting():
+    e = engine(EIGHT, budget=8)
+    e.steps = e.tokens_prefilled = e.tokens_decoded = 0
+    e.runner.kernel_times = None
+    e.add_request(range(22), 2, req_id="a")
+    for i in range(3):
+        e.add_request(range(22), 2, req_id=i, same_prompt_as="a")
+    assert e.stats()["waiting"] == 4
+    step(e)
+    assert (e.stats()["waiting"], e.stats()["running"]) == (3, 1)
+    step(e), step(e)
+    assert (e.stats()["waiting"], e.stats()["running"]) == (0, 4)
