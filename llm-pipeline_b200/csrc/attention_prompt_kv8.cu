@@ -55,7 +55,7 @@ struct Prompt8Params {
     const int* items;                                // [num_items][4]: request, first token, part | parts << 16, place of the item's sums
     float* partials;                                 // [places][nkv][256][P8_PART]
     long q_stride, out_stride, page_bytes;
-    int all_rows, table_stride, num_pages, nq, nkv, page_size, page_shift, window, tokens;
+    int table_stride, num_pages, nq, nkv, page_size, page_shift, window, tokens;
     float scale;
     int* error_flag;
 };
@@ -245,7 +245,7 @@ prompt_kv8_kernel(const __grid_constant__ CUtensorMap map, const Prompt8Params p
     const int G = p.nq / p.nkv;
     const int q_begin = p.q_start[r], q_len = p.q_start[r + 1] - q_begin;
     const int ctx = min(p.ctx_len[r], p.table_stride << p.page_shift), pos0 = p.ctx_len[r] - q_len;
-    const int ntok = min(min(q_len, p.all_rows - q_begin) - tok0, p.tokens);      // (no rows that are not there)
+    const int ntok = min(q_len - tok0, p.tokens);
     const int rows = ntok * G;
     const int* table = p.block_tables + (size_t)r * p.table_stride;
     // keys of the whole row tile, and this part's tiles of them; a row tile of 128 rows sees none beyond its last row's position
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(256) prompt_kv8_merge_kernel(const Prompt8Para
     pdl_wait();
     const int4 of = reinterpret_cast<const int4*>(shared)[blockIdx.y];
     const int kvh = blockIdx.z, index = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int G = p.nq / p.nkv, q_begin = p.q_start[of.x], ntok = min(min(p.q_start[of.x + 1], p.all_rows) - q_begin - of.y, p.tokens);
+    const int G = p.nq / p.nkv, q_begin = p.q_start[of.x], ntok = min(p.q_start[of.x + 1] - q_begin - of.y, p.tokens);
     if (index >= ntok * G) return;
     auto sums = [&](int part) { return p.partials + (((size_t)(of.w + part) * p.nkv + kvh) * (2 * P8_ROWS) + index) * P8_PART; };
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -680,8 +680,8 @@ LLMP_API int llmp_kv8_prompt_supports(int nq, int nkv, int d, int page_size) {
 LLMP_API int llmp_kv8_prompt_tokens(int nq, int nkv) { return nkv <= 0 || nq < nkv ? 0 : 2 * P8_ROWS / (nq / nkv); }
 LLMP_API long llmp_kv8_prompt_place_floats(int nkv) { return (long)nkv * 2 * P8_ROWS * P8_PART; }
 
-// all_rows: rows that both q and out have; items: [num_items][4] as in Prompt8Params; shared: [num_shared][4] as in prompt_kv8_merge_kernel; partials: the items' places.
-LLMP_API int llmp_kv8_prompt(const void* q, long q_stride, void* out, long out_stride, int all_rows, const void* pages, int num_pages, const int* block_tables,
+// items: [num_items][4] as in Prompt8Params; shared: [num_shared][4] as in prompt_kv8_merge_kernel; partials: the items' places.
+LLMP_API int llmp_kv8_prompt(const void* q, long q_stride, void* out, long out_stride, const void* pages, int num_pages, const int* block_tables,
                              int table_stride, const int* q_start, const int* ctx_len, const int* items, int num_items, const int* shared,
                              int num_shared, float* partials, int nq, int nkv, int page_size, int window, float scale, int* error_flag,
                              cudaStream_t stream) {
@@ -695,7 +695,7 @@ LLMP_API int llmp_kv8_prompt(const void* q, long q_stride, void* out, long out_s
     Prompt8Params p;
     p.q = (const bf16*)q; p.out = (bf16*)out; p.pages = (const unsigned char*)pages; p.block_tables = block_tables; p.q_start = q_start;
     p.ctx_len = ctx_len; p.items = items; p.partials = partials; p.q_stride = q_stride; p.out_stride = out_stride;
-    p.page_bytes = kv8_page_bytes(nkv, page_size, P8_D); p.all_rows = all_rows; p.table_stride = table_stride; p.num_pages = num_pages; p.nq = nq; p.nkv = nkv;
+    p.page_bytes = kv8_page_bytes(nkv, page_size, P8_D); p.table_stride = table_stride; p.num_pages = num_pages; p.nq = nq; p.nkv = nkv;
     p.page_size = page_size; p.page_shift = 31 - __builtin_clz((unsigned)page_size); p.window = window; p.tokens = llmp_kv8_prompt_tokens(nq, nkv);
     p.scale = scale; p.error_flag = error_flag;
     const int box_tokens = page_size < 32 ? page_size : 32;

@@ -129,7 +129,7 @@ _SIGNATURES = {
     "llmp_kv8_gather": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P],
     "llmp_kv8_decode": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
     "llmp_kv8_stream": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P, _P],
-    "llmp_kv8_prompt": [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P],
+    "llmp_kv8_prompt": [_P, _L, _P, _L, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P],
     "llmp_copy_pages": [_P, _I, _L, _P, _P, _I, _P],
 }
 _bound = {}
@@ -2510,8 +2510,8 @@ def kv8_prompt_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
                          page_size: int, window: int, scale: float) -> torch.Tensor:
     """Causal attention of a step's query rows (head size 128) over 8-bit pages. ``items`` int32 [n, 4]: request, first token, number of a
     part of the tile's keys | parts << 16, place of the part's sums; ``shared`` int32 [m, 4]: request, first token, parts, first place of
-    every tile that comes in parts (``ops.kv8.PromptPlan`` makes both; what they hold is not checked). Rows that q or out does not have are
-    left out. The scale may have any sign (``ops.kv8.prompt_attention``, which may go over unpacked pages, takes positive ones only)."""
+    every tile that comes in parts (``ops.kv8.PromptPlan`` makes both; what they and ``q_start`` hold is not checked: q and out need the
+    rows that they name). The scale may have any sign (``ops.kv8.prompt_attention``, which may go over unpacked pages, takes positive ones only)."""
     if not kv8_prompt_supports(q.dtype, num_heads, num_kv_heads, 128, page_size):
         if q.dtype != torch.bfloat16:
             raise KernelError("prompt attention over 8-bit pages takes bfloat16 queries")
@@ -2522,10 +2522,10 @@ def kv8_prompt_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
         raise KernelError("the lists of a prompt's items must be [n, 4]")
     if places < 0 or (places > 0) != (shared.shape[0] > 0):
         raise KernelError(f"{shared.shape[0]} shared tiles do not go with {places} places for their sums")
-    shape, width = q.shape, num_heads * 128
-    if len(shape) != 2 or shape[1] < width or q.stride(1) != 1 or (shape[0] > 1 and q.stride(0) != q_stride):
+    shape, stride, to, width = q.shape, q.stride(), out.shape, num_heads * 128
+    if len(shape) != 2 or shape[1] < width or stride[1] != 1 or (shape[0] > 1 and stride[0] != q_stride):
         raise KernelError("query rows must be [tokens, at least heads * 128] and lie q_stride apart")
-    if out.dtype != torch.bfloat16 or not out.is_contiguous() or out.dim() != 2 or out.shape[1] != width:
+    if out.dtype != torch.bfloat16 or len(to) != 2 or to[1] != width or not out.is_contiguous():
         raise KernelError("prompt attention over 8-bit pages gives contiguous bfloat16 [tokens, heads * 128]")
     R, table = ctx_len.numel(), block_tables.shape
     if len(table) != 2 or table[0] != R or table[1] == 0 or q_start.numel() != R + 1:
@@ -2535,7 +2535,7 @@ def kv8_prompt_attention(q: torch.Tensor, q_stride: int, out: torch.Tensor, page
     _kv8_pages(pages, num_kv_heads, 128, page_size)
     _on_current_device(q, out, pages, block_tables, q_start, ctx_len, items, shared)
     partials = torch.empty(places * kv8_prompt_sizes(num_heads, num_kv_heads)[1], dtype=torch.float32, device=q.device) if places else None
-    _call("llmp_kv8_prompt", q.data_ptr(), q_stride, out.data_ptr(), width, min(shape[0], out.shape[0]), pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
+    _call("llmp_kv8_prompt", q.data_ptr(), q_stride, out.data_ptr(), width, pages.data_ptr(), pages.shape[0], block_tables.data_ptr(),
           table[1], q_start.data_ptr(), ctx_len.data_ptr(), items.data_ptr(), items.shape[0], shared.data_ptr() if places else None,
           shared.shape[0], None if partials is None else partials.data_ptr(), num_heads, num_kv_heads, page_size, window, scale,
           error_flag().data_ptr(), _stream())
