@@ -4,7 +4,8 @@ bfloat16 queries of head size 128 go to a kernel that reads the pages as they ar
 faster: few queries over many keys above all (``reads_pages_directly``). For all others the pages that a step's portions see are
 unpacked into a workspace of the query's type, laid out as ordinary pages, and the attention kernels of ordinary pages run over it
 (``kernels.paged_attention``): a page's values are exact in either type (the scales are powers of two), so the result is exactly what
-they give for a cache that holds these values. A value that is no number makes the whole rows of its head's group that see its token no
+they give for a cache that holds these values, their weights in bfloat16 included (2^-8 of sum w |v|; the kernel that reads the pages has
+them in half precision, 2^-11). A value that is no number makes the whole rows of its head's group that see its token no
 numbers either way, and no others (single tokens: the entries of its column)."""
 
 from __future__ import annotations
@@ -69,7 +70,9 @@ def reads_pages_directly(starts: Sequence[int], q_lens: Sequence[int], first_req
     18 and the longer of 2.75 a key tile of the longest part and 3.2 for every key tile an SM has, against 8, 1.9 for every 1,000 tokens of
     the pages, and the longer of 2.8 a key tile of the longest item and 1.3 for every key tile an SM has, with up to 18 for the end. Measured
     (direct, unpacked), 32 query heads: 40 new tokens behind 8,000 31, 71; 128 behind 2,000 29, 48; 512 behind 8,000 113, 131; 1,024 behind
-    8,000 206, 209; 2,048 new ones 66, 70; 64 behind 500 24, 22; 1,000 new ones 35, 31; 4,000 new ones 200, 181; 2,048 behind 14,000 649, 606."""
+    8,000 206, 209; 2,048 new ones 65, 66; 64 behind 500 24, 21; 1,000 new ones 34, 30; 4,000 new ones 195, 179; 2,048 behind 14,000 644, 638. Other
+    groups (8, 16 and 64 heads on 8, 32 on 4, 9 and 16 on 1), the worst of nine mixes of lengths each: 64 behind 500 on 16 and 8 heads 18.5, 21.9 (taken:
+    unpacked), 512 behind 8,000 on 32 and 4 110, 125 (unpacked), 1,000 new ones on 9 and 1 29.6, 26.3 (direct)."""
     group = num_heads // num_kv_heads
     wide = tiles_of(starts, q_lens, first_request, max(1, 256 // group), window)
     if not wide:
@@ -110,7 +113,8 @@ class PromptPlan:
         self.first_request = first_request
         self.rows = sum(self.q_lens)
         # The first row where all portions are single tokens: the kernel for those takes them (behind 4,934 tokens, 3 requests of 12 and 2
-        # heads of 64: 132 us as portions, whose keys only some sizes share among blocks, 14 as single tokens).
+        # heads of 64: 132 us as portions, whose keys only some sizes share among blocks, 14 as single tokens). A step of the engine has its
+        # single tokens in front, where `first_request` leaves them out.
         self.single = sum(self.q_lens[:first_request]) if all(n == 1 for n in self.q_lens[first_request:]) else None
         self.longest = max((s + n for s, n in zip(self.starts, self.q_lens)), default=0)
         self.page_bytes = 2 * num_kv_heads * page_size * head_dim * dtype.itemsize
