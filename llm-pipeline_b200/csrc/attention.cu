@@ -143,9 +143,11 @@ __global__ void __launch_bounds__(ATT_THREADS) paged_attention_kernel(const Attn
             const float s = Ss[rr * (ATT_KEYS + 1) + lane];
             const float m_old = row_m[rr];
             const float m_new = fmaxf(m_old, warp_max(s));
-            // masked keys have weight 0; a score that is no number keeps its own, also where none of the row is a number
-            const float pr = s == -INFINITY ? 0.f : expf(s - (m_new > -INFINITY ? m_new : 0.f));
-            const float alpha = m_new > -INFINITY ? expf(m_old - m_new) : 1.f;      // 0 when nothing was seen before
+            float pr = s == -INFINITY ? 0.f : s, alpha = 1.f;      // no maximum: masked keys, and scores that are no numbers
+            if (m_new > -INFINITY) {
+                pr = expf(s - m_new);          // exp(-inf) = 0 for masked keys
+                alpha = expf(m_old - m_new);   // 0 when nothing was seen before
+            }
             const float sum = warp_sum(pr);
             Ss[rr * (ATT_KEYS + 1) + lane] = pr;
             __syncwarp();

@@ -378,7 +378,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_pages, const
                     for (int i = 0; i < 32; ++i) part[(size_t)(c + i) * FA_ROWS + tid] = __uint_as_float(a[i]);   // column by column: the lanes of a warp write one line
                 }
             }
-            part[FA_ROWS * FA_D + tid] = num_key_tiles > 0 ? m_used : -INFINITY;
+            // (a sum that is no number may have come without a maximum: its item then has a weight that is none, and the others none)
+            part[FA_ROWS * FA_D + tid] = num_key_tiles > 0 ? (l_run == l_run ? m_used : INFINITY) : -INFINITY;
             part[FA_ROWS * FA_D + FA_ROWS + tid] = num_key_tiles > 0 ? l_run : 0.f;
             __threadfence();                                         // the sums are visible before the count is
             asm volatile("bar.sync 1, 128;\n" ::: "memory");
@@ -397,10 +398,8 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_pages, const
                 }
 #pragma unroll
                 for (int x = 0; x < FA_MAX_SEGMENTS; ++x) {
-                    // (an item without a maximum saw no key, its sum is 0, or none whose score is a number: that sum counts)
-                    const float sum = x < nseg ? __ldcg(first + (size_t)x * p.nkv * FA_PART + FA_ROWS * FA_D + FA_ROWS + tid) : 0.f;
-                    wgt[x] = wgt[x] > -INFINITY ? fa_ex2(wgt[x] - m) : (sum != 0.f ? 1.f : 0.f);
-                    if (wgt[x] != 0.f) l = fmaf(sum, wgt[x], l);
+                    wgt[x] = wgt[x] > -INFINITY ? fa_ex2(wgt[x] - m) : 0.f;
+                    if (x < nseg && wgt[x] != 0.f) l = fmaf(__ldcg(first + (size_t)x * p.nkv * FA_PART + FA_ROWS * FA_D + FA_ROWS + tid), wgt[x], l);
                 }
                 const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
